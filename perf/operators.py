@@ -226,12 +226,10 @@ def prepare(case, seed):
         shape = (L, t["table2"].numel(), Hkv, page, HD)
         s["k2"], s["v2"] = (torch.zeros(shape, dtype=BF, device=DEV) for _ in range(2))
         if own:
-            from specfold_amd import _lib
             s["cache"] = _cache(L, Hkv, page, s.pop("k"), s.pop("v"), t["table"], case["length"])
             s["into"] = _cache(L, Hkv, page, s.pop("k2"), s.pop("v2"), t["table2"], 0)
             s["kept"] = torch.empty(L, Hkv, keep, dtype=torch.int32, device=DEV)
             s["mass2"] = torch.empty(L, Hkv, keep, device=DEV)
-            s["ws"] = _ws(_lib.kv_evict_workspace_bytes(L, Hkv, case["length"], keep))
         return s
     seqs, q = _cached(case, seed)
     s = dict(case=dict(case), q=q)
@@ -246,10 +244,8 @@ def prepare(case, seed):
         from specfold_amd.kv_cache import PagedBatch
         s["batch"] = PagedBatch([_cache(1, Hkv, case["page"], x["k"], x["v"], x["table"], x["P"])
                                  for x in seqs], [x["n"] for x in seqs])
-        size = (_lib.attn_window_workspace_bytes if case["kind"] == "attend"
-                else _lib.attn_key_mass_workspace_bytes)
-        s["ws"] = _ws(size(s["batch"], H, block=case["block"], window=case["window"],
-                           sinks=case["sinks"]))
+        s["ws"] = _ws(_lib.attn_window_workspace_bytes(q.shape[0], H) if case["kind"] == "attend"
+                      else _lib.attn_key_mass_workspace_bytes(sum(x["P"] for x in seqs), Hkv))
     else:
         s["seqs"] = seqs
     return s
@@ -293,7 +289,7 @@ def _run_own(s):
     H = MODELS[case["model"]][0]
     if case["kind"] == "evict":
         s["cache"].evict(s["mass"], case["keep"], sinks=case["sinks"], recent=case["recent"],
-                         into=s["into"], kept=s["kept"], mass_out=s["mass2"], workspace=s["ws"])
+                         into=s["into"], kept=s["kept"], mass_out=s["mass2"])
         return {"k": s["into"].k_pages, "v": s["into"].v_pages, "kept": s["kept"],
                 "mass": s["mass2"]}
     mask = dict(block=case["block"], window=case["window"], sinks=case["sinks"])

@@ -78,7 +78,8 @@ const char* sf_status_string(int status);
  * 12: SF_GATE_DEFER_COMPACT and sf_qkv_rope_gated (the compaction in the QKV GEMM).
  * 13: sf_head_logits_rows (the head for the rows a decode step reads).
  * 14: sf_decode_facts; sf_attn_rows / sf_attn_prefix_block take NULL o32, m_tab, z_tab
- *     (sf_attn_chunk joined it: an addition, nothing that was there changed). */
+ *     (sf_attn_chunk, sf_attn_window, sf_attn_key_mass and sf_kv_evict joined it:
+ *     additions, nothing that was there changed). */
 int sf_abi_version(void);
 
 /*
@@ -474,6 +475,101 @@ int sf_decode_facts(int64_t* x_t, int L, int plen, int bl, int sbs, int s0, long
                     long long stop_id, const uint16_t* conf, const int64_t* x_1, float threshold,
                     const int64_t* const* states, int n_states, int8_t* unmask, int64_t* facts,
                     void* stream);
+
+/* ---- a bounded prefix cache ------------------------------------------------------
+ * Attention that sees a window and a few first tokens, the attention weight every
+ * cached key got, and the eviction of keys that got little.  No counterpart in the
+ * reference, whose prefix cache only grows (specfold/generate/fastdllm_v2_generation.py:
+ * 557-575).
+ *
+ * One sequence of a call: its cache and its new rows, the rows' own K and V in the
+ * cache already (sf_kv_append) as the last `rows` of its `length` keys.  A host array of
+ * these describes a call; the rows of sequence s follow those of s - 1 in q, o and lse.
+ */
+typedef struct sf_kv_seq {
+  const uint16_t* k;          /* cache, as cache_k / cache_v of sf_attn_chunk */
+  const uint16_t* v;          /* (sf_attn_key_mass does not read it: may be NULL there) */
+  const int32_t* page_table;  /* NULL: contiguous, element (h, t, d) at h * head_stride + t * hd + d */
+  const float* mass_in;       /* sf_attn_key_mass only: [Hkv][mass_in_stride], NULL: zeros */
+  float* mass_out;            /* sf_attn_key_mass only: [Hkv][mass_out_stride]; may be mass_in */
+  long long page_stride;
+  long long head_stride;
+  long long mass_in_stride;
+  long long mass_out_stride;
+  int length;                 /* cached keys, the new rows' own included */
+  int rows;                   /* new rows, 0 .. length */
+  int pages;                  /* pages of the pool: a page id outside [0, pages) is taken as page 0 */
+  int reserved;               /* 0 */
+} sf_kv_seq;
+
+/*
+ * Attention of the new rows of up to 32 sequences in one call.  Row m of a sequence of
+ * n rows is at position p = length - n + m and sees the keys t below the end of its own
+ * block of `block` rows (blocks counted from row 0, the last may be short; block = 1:
+ * causal) that are among the first `sinks` or not more than window - 1 positions before
+ * p (t > p - window); window = 0: every key below that end.
+ *   o[m]   = sum over the seen keys of softmax(scaling * q . k) v, bf16, [rows][H*hd]
+ *   lse[m] = ln sum exp(scaling * q . k), fp32, [rows][H]; may be NULL
+ * (rows: those of all sequences; rows of q, o and lse behind them are not touched.)
+ * Scores, maxima, sums and accumulators are fp32; the softmax weights go to the value
+ * product as bf16 (half a step, 2^-8 of each weight; the sums lse is made of are not
+ * rounded).  Keys and values that a row does not see never reach it, NaN and inf among
+ * them.  Results do not depend on the order of pages or of workgroups.
+ * workspace: sf_attn_window_workspace_bytes(rows, H) bytes, 16-byte aligned; calls that
+ * share one must not overlap (two captured graphs that may replay at once need two).
+ * Limits: hd == 128, H % Hkv == 0, H/Hkv <= 16, 1 <= n_seqs <= 32, 0 <= rows <= length
+ * <= 32768 (each sequence), block >= 1, window >= 0, sinks >= 0; page_size 16, 32, 64 or
+ * 128 where a page_table is given; strides multiples of 8 elements, 16-byte aligned
+ * pointers.
+ */
+size_t sf_attn_window_workspace_bytes(int rows, int H);
+int sf_attn_window(const uint16_t* q, const sf_kv_seq* seqs, int n_seqs, int page_size, int block,
+                   int window, int sinks, int H, int Hkv, int hd, float scaling, uint16_t* o,
+                   float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The attention weight every cached key got from the same rows:
+ *   mass_out[h][t] = decay * mass_in[h][t] + sum over the rows that see t and the H/Hkv
+ *                    q-heads of kv head h of exp(scaling * q . k - lse),   t < length
+ * with lse as sf_attn_window wrote it; entries at and behind length are not touched.
+ * fp32 sums in a fixed order (no atomics).  Masks and limits as sf_attn_window;
+ * 0 <= decay <= 1.  workspace: sf_attn_key_mass_workspace_bytes(keys, Hkv) bytes, keys =
+ * the sum of the sequences' lengths, 16-byte aligned.
+ */
+size_t sf_attn_key_mass_workspace_bytes(int keys, int Hkv);
+int sf_attn_key_mass(const uint16_t* q, const float* lse, const sf_kv_seq* seqs, int n_seqs,
+                     int page_size, int block, int window, int sinks, int H, int Hkv, int hd,
+                     float scaling, float decay, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/*
+ * Eviction: of the P keys of every (layer, kv head) keep the first `sinks`, the last
+ * `recent` and, of the others, those with the largest mass (equal mass: the lower index;
+ * NaN above every number), `keep` in all, and move their K and V rows to slots 0 ..
+ * keep - 1 of `to` in ascending order.  `to` is `from` itself (the same mapping: in
+ * place) or shares no page with it.
+ *   kept[l][h][j]  int32, the old slot of slot j
+ *   mass_out       the kept keys' mass, [l][h] rows at mass_out_layer / _head strides;
+ *                  may be NULL; where it is `mass` itself (same strides), entries
+ *                  keep .. P - 1 are set to 0
+ * Keys keep the RoPE angles they were appended with.  Limits: hd == 128, 1 <= P <= 32768,
+ * sinks + recent <= keep <= P, keep >= 1; page sizes and alignment as sf_attn_window, a
+ * page_table in both; an id outside [0, pages) is read as page 0 and not written.
+ */
+typedef struct sf_kv_pages {
+  uint16_t* k;                /* [layers] at layer_stride, pages at page_stride, ... */
+  uint16_t* v;
+  const int32_t* page_table;  /* shared by the layers */
+  long long layer_stride;
+  long long page_stride;
+  long long head_stride;
+  int page_size;
+  int pages;
+} sf_kv_pages;
+int sf_kv_evict(const float* mass, long long mass_layer, long long mass_head, int layers, int Hkv,
+                int hd, int P, int sinks, int recent, int keep, const sf_kv_pages* from,
+                const sf_kv_pages* to, int32_t* kept, float* mass_out, long long mass_out_layer,
+                long long mass_out_head, void* stream);
 
 #ifdef __cplusplus
 }

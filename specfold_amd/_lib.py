@@ -9,6 +9,7 @@ pointers and the current HIP stream.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from pathlib import Path
 from typing import Optional
@@ -29,6 +30,22 @@ _i = ctypes.c_int
 _f = ctypes.c_float
 _ll = ctypes.c_longlong
 _sz = ctypes.c_size_t
+
+
+
+class KVSeq(ctypes.Structure):
+    """sf_kv_seq: one sequence's cache and new rows."""
+    _fields_ = [("k", _vp), ("v", _vp), ("page_table", _vp), ("mass_in", _vp), ("mass_out", _vp),
+                ("page_stride", _ll), ("head_stride", _ll), ("mass_in_stride", _ll),
+                ("mass_out_stride", _ll), ("length", _i), ("rows", _i), ("pages", _i),
+                ("reserved", _i)]
+
+
+class KVPages(ctypes.Structure):
+    """sf_kv_pages: every layer's pages of a cache."""
+    _fields_ = [("k", _vp), ("v", _vp), ("page_table", _vp), ("layer_stride", _ll),
+                ("page_stride", _ll), ("head_stride", _ll), ("page_size", _i), ("pages", _i)]
+
 
 # name -> (restype, argtypes); mirrors include/specfold_amd.h
 SIGNATURES = {
@@ -57,6 +74,14 @@ SIGNATURES = {
     "sf_attn_chunk_workspace_bytes": (_sz, [_i, _i]),
     "sf_attn_chunk": (_i, [_vp, _vp, _vp, _vp, _i, _i, _ll, _ll, _i, _i, _i, _i, _i, _f, _vp, _vp,
                            _sz, _vp]),
+    "sf_attn_window_workspace_bytes": (_sz, [_i, _i]),
+    "sf_attn_window": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp, _sz,
+                            _vp]),
+    "sf_attn_key_mass_workspace_bytes": (_sz, [_i, _i]),
+    "sf_attn_key_mass": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _f, _vp, _sz,
+                              _vp]),
+    "sf_kv_evict": (_i, [_vp, _ll, _ll, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _ll, _ll,
+                         _vp]),
     "sf_chain_correct": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f,
                               _vp, _vp, _vp, _vp, _vp]),
     "sf_kv_append": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _ll, _ll, _i, _vp]),
@@ -433,6 +458,124 @@ def attn_chunk(q_buf, cache_k, cache_v, page_table, P, page_size, page_stride, h
                               float(scaling), _ptr(o_bf), _ptr(workspace), workspace.numel(),
                               _stream(stream))
     _check(st, "sf_attn_chunk")
+
+
+def attn_window_workspace_bytes(rows: int, H: int) -> int:
+    return int(load().sf_attn_window_workspace_bytes(rows, H))
+
+
+def attn_key_mass_workspace_bytes(keys: int, Hkv: int) -> int:
+    """keys: the sum of the sequences' lengths."""
+    return int(load().sf_attn_key_mass_workspace_bytes(keys, Hkv))
+
+
+@contextlib.contextmanager
+def _on(t: torch.Tensor, **others):
+    """The device of ``t`` current, the other tensors (None allowed) checked to be on it."""
+    for nm, o in others.items():
+        if o is not None and o.device != t.device:
+            raise ValueError(f"{nm}: on {o.device}, expected {t.device}")
+    if t.device.type != "cuda" or t.device.index == torch.cuda.current_device():
+        yield
+    else:
+        with torch.cuda.device(t.device):
+            yield
+
+
+def attn_window(q, batch, li, H, scaling, o, workspace, lse=None, block: int = 1, window: int = 0,
+                sinks: int = 0, stream=None) -> None:
+    """Attention of the new rows of a PagedBatch (their K/V the last keys of their caches'
+    layer ``li``): every row sees the keys below its block's end (block = 1: causal) that
+    are among the first ``sinks`` or less than ``window`` positions before it (0: all).
+    q, o [rows, H*hd] bf16, lse [rows, H] fp32 or None; rows of theirs behind the batch's
+    are not touched (sf_attn_window)."""
+    rows, hd = batch.num_rows, batch.hd
+    _need(q, "q", torch.bfloat16, min_numel=rows * H * hd)
+    _need(o, "o", torch.bfloat16, min_numel=rows * H * hd)
+    if lse is not None:
+        _need(lse, "lse", torch.float32, min_numel=rows * H, align=4)
+    _need(workspace, "workspace", torch.uint8, min_numel=attn_window_workspace_bytes(rows, H))
+    seqs = batch.seqs(li)
+    with _on(q, o=o, lse=lse, workspace=workspace, caches=batch):
+        st = load().sf_attn_window(_ptr(q), seqs, len(seqs), batch.page_size, block, window, sinks,
+                                   H, batch.Hkv, hd, float(scaling), _ptr(o), _ptr(lse),
+                                   _ptr(workspace), workspace.numel(), _stream(stream))
+    _check(st, "sf_attn_window")
+
+
+def attn_key_mass(q, lse, batch, li, H, scaling, mass, workspace, mass_in=None, decay: float = 1.0,
+                  block: int = 1, window: int = 0, sinks: int = 0, stream=None) -> None:
+    """The attention weight every cached key got from the batch's rows: mass[s] [Hkv, >= length
+    of sequence s] fp32 = decay * mass_in[s] (``mass_in`` None: zeros; it may be ``mass``)
+    + the weights exp(scaling * q.k - lse) summed over the rows that see the key and the
+    q-heads of its kv head (sf_attn_key_mass).  q, lse and the mask as in attn_window."""
+    rows, hd = batch.num_rows, batch.hd
+    _need(q, "q", torch.bfloat16, min_numel=rows * H * hd)
+    _need(lse, "lse", torch.float32, min_numel=rows * H, align=4)
+    seqs = batch.seqs(li)
+    total = sum(s.length for s in seqs)
+    _need(workspace, "workspace", torch.uint8,
+          min_numel=attn_key_mass_workspace_bytes(total, batch.Hkv))
+    for name, ts in (("mass", mass), ("mass_in", mass_in)):
+        if ts is None:
+            continue
+        if len(ts) != len(seqs):
+            raise ValueError(f"{name}: one tensor per sequence, got {len(ts)} for {len(seqs)}")
+        for s, t in zip(seqs, ts):
+            if t.dtype != torch.float32 or t.dim() != 2 or t.shape[0] != batch.Hkv or \
+                    t.shape[1] < s.length or t.stride(1) != 1:
+                raise ValueError(f"{name}: expected float32 [{batch.Hkv}, >= {s.length}] with "
+                                 f"contiguous rows, got {t.dtype} {tuple(t.shape)}")
+            if t.device != q.device:
+                raise ValueError(f"{name}: on {t.device}, expected {q.device}")
+            if name == "mass":
+                s.mass_out, s.mass_out_stride = t.data_ptr(), t.stride(0)
+                s.mass_in, s.mass_in_stride = None, 0
+            else:
+                s.mass_in, s.mass_in_stride = t.data_ptr(), t.stride(0)
+    with _on(q, lse=lse, workspace=workspace, caches=batch):
+        st = load().sf_attn_key_mass(_ptr(q), _ptr(lse), seqs, len(seqs), batch.page_size, block,
+                                     window, sinks, H, batch.Hkv, hd, float(scaling), float(decay),
+                                     _ptr(workspace), workspace.numel(), _stream(stream))
+    _check(st, "sf_attn_key_mass")
+
+
+def kv_evict(mass, length: int, keep: int, sinks: int, recent: int, src, dst, kept,
+             mass_out=None, stream=None) -> None:
+    """Keep ``keep`` of the first ``length`` keys of every layer and kv head of the paged
+    cache ``src`` -- the first ``sinks``, the last ``recent``, then those with the largest
+    mass [layers, Hkv, >= length] fp32 -- and move them to the front of ``dst`` (``src``
+    itself: in place).  kept [layers, Hkv, keep] int32: their old slots; mass_out [layers,
+    Hkv, >= keep] fp32 (or None; ``mass`` itself: moved in place, the rest zeroed).  The
+    caches' lengths are the caller's (PagedKVCache.evict)."""
+    L, Hkv, hd = src.num_layers, src.Hkv, src.hd
+    if (dst.num_layers, dst.Hkv, dst.hd) != (L, Hkv, hd):
+        raise ValueError("the caches' layers, kv heads and head sizes differ")
+    if length > src.capacity or keep > dst.capacity:
+        raise ValueError(f"{length} -> {keep} keys exceed the caches' capacities "
+                         f"{src.capacity}, {dst.capacity}")
+    _need(kept, "kept", torch.int32, numel=L * Hkv * keep, align=4)
+    for nm, t, n in (("mass", mass, length), ("mass_out", mass_out, keep)):
+        if t is None and nm == "mass_out":
+            continue
+        if t.dtype != torch.float32 or t.dim() != 3 or tuple(t.shape[:2]) != (L, Hkv) or \
+                t.shape[2] < n or t.stride(2) != 1:
+            raise ValueError(f"{nm}: expected float32 [{L}, {Hkv}, >= {n}] with contiguous rows, "
+                             f"got {t.dtype} {tuple(t.shape)}")
+    pages = []
+    for c in (src, dst):
+        _need(c.k_pages, "k_pages", torch.bfloat16)
+        _need(c.v_pages, "v_pages", torch.bfloat16)
+        pages.append(KVPages(c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.page_table.data_ptr(),
+                             c.k_pages.stride(0), c.k_pages.stride(1), c.k_pages.stride(2),
+                             c.page_size, c.num_pages))
+    with _on(mass, kept=kept, mass_out=mass_out, src=src.k_pages, dst=dst.k_pages):
+        st = load().sf_kv_evict(
+            _ptr(mass), mass.stride(0), mass.stride(1), L, Hkv, hd, length, sinks, recent, keep,
+            ctypes.byref(pages[0]), ctypes.byref(pages[1]), _ptr(kept), _ptr(mass_out),
+            0 if mass_out is None else mass_out.stride(0),
+            0 if mass_out is None else mass_out.stride(1), _stream(stream))
+    _check(st, "sf_kv_evict")
 
 
 def chain_correct(q_buf, kv_buf, src, par, rec, seg, segcnt, B1, N, H, Hkv, hd, scaling,

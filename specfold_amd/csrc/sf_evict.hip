@@ -1,0 +1,220 @@
+// Eviction from the prefix cache by accumulated attention weight (sf_kv_evict).  No
+// counterpart in the reference, whose cache only grows.
+//
+// Of the P keys of a (layer, kv head): the first `sinks`, the last `recent` and the
+// k = keep - sinks - recent others with the largest mass, equal ones by the lower index.
+//  * select: one workgroup per (layer, kv head).  The masses are mapped to unsigned
+//    integers of the same order and stay in registers; the k-th largest value is built
+//    bit by bit from the top (how many are >= the candidate), exact and without atomics;
+//    two ballot scans number the ties and the kept keys in index order.
+//  * move: the kept rows to slots 0 .. keep - 1, ascending.  Slot j takes a row from a
+//    slot >= j, so a workgroup that goes up the slots, every row of a tile read before
+//    the tile is written, may move in place.
+#include "sf_common.h"
+
+namespace {
+
+constexpr int kHD = 128;
+constexpr int kMaxKeys = 32768;
+constexpr int kSelThreads = 1024;
+constexpr int kSelWaves = kSelThreads / 64;
+
+// The order of a float as an unsigned integer: NaN above all, -0 as 0.
+SF_DEV uint32_t order_of(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+SF_DEV int block_sum(int v, int* s_red) {
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  int t = 0;
+  for (int w = 0; w < kSelWaves; ++w) t += s_red[w];
+  return t;
+}
+
+template <int PER>   // keys of a thread: t = i * 1024 + tid
+__global__ __launch_bounds__(kSelThreads) void sf_evict_select_kernel(
+    const float* mass, long long mass_layer, long long mass_head, int Hkv, int P, int sinks,
+    int recent, int keep, int32_t* __restrict__ kept, float* mass_out, long long out_layer,
+    long long out_head, int zero_to) {
+  __shared__ int s_red[kSelWaves];
+  __shared__ int s_cnt[PER * kSelWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int l = blockIdx.x / Hkv, h = blockIdx.x - l * Hkv;
+  const float* in = mass + l * mass_layer + h * mass_head;
+  const int last = P - recent;
+  uint32_t key[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = i * kSelThreads + tid;
+    // only the keys in between compete
+    key[i] = t >= sinks && t < last ? order_of(in[t]) : 0u;
+  }
+  const int need = keep - sinks - recent;   // <= last - sinks
+  uint32_t thr = 0;                         // the need-th largest
+  if (need > 0) {
+    for (int b = 31; b >= 0; --b) {
+      const uint32_t cand = thr | (1u << b);
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) n += key[i] >= cand ? 1 : 0;
+      if (block_sum(n, s_red) >= need) thr = cand;
+    }
+  }
+  int above = 0;
+  uint32_t keeps = 0, equal = 0;   // bit i: key i of this thread
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = i * kSelThreads + tid;
+    const bool mid = t >= sinks && t < last;
+    if (t < P && (!mid || (need > 0 && key[i] > thr))) keeps |= 1u << i;
+    if (mid && need > 0 && key[i] == thr) equal |= 1u << i;
+    above += mid && need > 0 && key[i] > thr ? 1 : 0;
+  }
+  const int ties = need - block_sum(above, s_red);   // of the equal ones the first `ties`
+  // index-order numbering of the flagged keys: s_cnt holds, for each 64 of them, how
+  // many are flagged in front
+  auto scan = [&](uint32_t bits) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const unsigned long long b = __ballot(bits >> i & 1u);
+      if (lane == 0) s_cnt[i * kSelWaves + wv] = __popcll(b);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int at = 0;
+      for (int j = 0; j < PER * kSelWaves; ++j) {
+        const int n = s_cnt[j];
+        s_cnt[j] = at;
+        at += n;
+      }
+    }
+    __syncthreads();
+  };
+  const unsigned long long below = (1ull << lane) - 1;
+  scan(equal);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const unsigned long long b = __ballot(equal >> i & 1u);
+    const int rank = s_cnt[i * kSelWaves + wv] + __popcll(b & below);
+    if ((equal >> i & 1u) && rank < ties) keeps |= 1u << i;
+  }
+  scan(keeps);
+  int32_t* kp = kept + (size_t)blockIdx.x * keep;
+  float* mo = mass_out ? mass_out + l * out_layer + h * out_head : nullptr;
+  // the masses again (in place they are all read before the first is written)
+  float val[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) val[i] = mo && (keeps >> i & 1u) ? in[i * kSelThreads + tid] : 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sf_pin(val[i]);
+  sf_wait_vm_loads();
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = i * kSelThreads + tid;
+    const unsigned long long b = __ballot(keeps >> i & 1u);
+    if (keeps >> i & 1u) {
+      const int rank = s_cnt[i * kSelWaves + wv] + __popcll(b & below);
+      kp[rank] = t;
+      if (mo) mo[rank] = val[i];
+    }
+    if (mo && t >= keep && t < zero_to) mo[t] = 0.f;
+  }
+}
+
+struct Pages {
+  uint16_t* base;
+  const int32_t* table;
+  long long layer_stride, page_stride, head_stride;
+  int page_size, pages;
+};
+SF_DEV long long slot_off(const Pages& p, int l, int h, int t, bool& ok) {
+  const int lp = t / p.page_size;
+  const int id = p.table[lp];
+  ok = id >= 0 && id < p.pages;
+  return l * p.layer_stride + (ok ? id : 0) * p.page_stride + h * p.head_stride +
+         (long long)(t - lp * p.page_size) * kHD;
+}
+
+constexpr int kMoveThreads = 256;
+constexpr int kMoveRows = 8;   // rows of a thread in a tile: 16 * 8 rows a tile
+__global__ __launch_bounds__(kMoveThreads) void sf_evict_move_kernel(
+    Pages fk, Pages fv, Pages tk, Pages tv, const int32_t* __restrict__ kept, int Hkv, int keep) {
+  const int l = blockIdx.x / Hkv, h = blockIdx.x - l * Hkv;
+  const Pages from = blockIdx.y ? fv : fk, to = blockIdx.y ? tv : tk;
+  const int32_t* kp = kept + (size_t)blockIdx.x * keep;
+  const int unit = threadIdx.x & 15, r = threadIdx.x >> 4;
+  for (int j0 = 0; j0 < keep; j0 += 16 * kMoveRows) {
+    sf_u32x4 w[kMoveRows];
+#pragma unroll
+    for (int i = 0; i < kMoveRows; ++i) {
+      const int j = min(j0 + 16 * i + r, keep - 1);
+      bool ok;
+      const long long at = slot_off(from, l, h, kp[j], ok);
+      w[i] = *reinterpret_cast<const sf_u32x4*>(from.base + at + unit * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < kMoveRows; ++i) sf_pin(w[i]);
+    sf_wait_vm_loads();
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMoveRows; ++i) {
+      const int j = j0 + 16 * i + r;
+      bool ok;
+      const long long at = slot_off(to, l, h, min(j, keep - 1), ok);
+      if (j < keep && ok) *reinterpret_cast<sf_u32x4*>(to.base + at + unit * 8) = w[i];
+    }
+  }
+}
+
+int check_pages(const sf_kv_pages* p, int keys) {
+  if (!p || !p->k || !p->v || !p->page_table) return SF_ERR_ARG;
+  if (reinterpret_cast<uintptr_t>(p->k) % 16 || reinterpret_cast<uintptr_t>(p->v) % 16)
+    return SF_ERR_ARG;
+  if (p->page_size != 16 && p->page_size != 32 && p->page_size != 64 && p->page_size != 128)
+    return SF_ERR_SHAPE;
+  if (p->pages < 1 || (long long)p->pages * p->page_size < keys) return SF_ERR_SHAPE;
+  if (p->layer_stride % 8 || p->page_stride % 8 || p->head_stride % 8) return SF_ERR_SHAPE;
+  return SF_OK;
+}
+
+}  // namespace
+
+extern "C" int sf_kv_evict(const float* mass, long long mass_layer, long long mass_head,
+                           int layers, int Hkv, int hd, int P, int sinks, int recent, int keep,
+                           const sf_kv_pages* from, const sf_kv_pages* to, int32_t* kept,
+                           float* mass_out, long long mass_out_layer, long long mass_out_head,
+                           void* stream) {
+  if (!mass || !kept) return SF_ERR_ARG;
+  if (hd != kHD || layers < 1 || Hkv < 1 || P < 1 || P > kMaxKeys) return SF_ERR_SHAPE;
+  if (keep < 1 || keep > P || sinks < 0 || recent < 0 || sinks > keep || recent > keep - sinks)
+    return SF_ERR_SHAPE;
+  int st = check_pages(from, P);
+  if (st == SF_OK) st = check_pages(to, keep);
+  if (st != SF_OK) return st;
+  if (mass_out == mass && (mass_out_layer != mass_layer || mass_out_head != mass_head))
+    return SF_ERR_ARG;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+#define SF_EVICT_SELECT(PER)                                                                    \
+  hipLaunchKernelGGL((sf_evict_select_kernel<PER>), dim3(layers * Hkv), dim3(kSelThreads), 0, s, \
+                     mass, mass_layer, mass_head, Hkv, P, sinks, recent, keep, kept, mass_out,   \
+                     mass_out_layer, mass_out_head, mass_out == mass ? P : 0)
+  if (P <= 4 * kSelThreads) SF_EVICT_SELECT(4);
+  else if (P <= 16 * kSelThreads) SF_EVICT_SELECT(16);
+  else SF_EVICT_SELECT(32);
+#undef SF_EVICT_SELECT
+  auto pages = [](const sf_kv_pages* p, uint16_t* base) {
+    return Pages{base, p->page_table, p->layer_stride, p->page_stride, p->head_stride,
+                 p->page_size, p->pages};
+  };
+  hipLaunchKernelGGL(sf_evict_move_kernel, dim3(layers * Hkv, 2), dim3(kMoveThreads), 0, s,
+                     pages(from, from->k), pages(from, from->v), pages(to, to->k),
+                     pages(to, to->v), kept, Hkv, keep);
+  return sf_launch_status();
+}

@@ -42,7 +42,8 @@ from typing import Dict, List, Optional, Tuple
 import torch
 
 from specfold_amd import _lib
-from specfold_amd.kv_cache import ContiguousMirror, PagedKVCache, cache_length, prefix_view
+from specfold_amd.kv_cache import (ContiguousMirror, PagedBatch, PagedKVCache, cache_length,
+                                   cache_position, prefix_view)
 
 
 @contextlib.contextmanager
@@ -246,8 +247,8 @@ class _Batch:
                 dst.copy_(q.reshape(1, N).to(dtype=torch.float32).expand(b, N))
 
     def refresh_positions(self) -> None:
-        """pos0_branch[b] = its sequence's prefix length, read on the device."""
-        torch.cat([c.length_dev.expand(b) if c is not None else self._zeros[:b]
+        """pos0_branch[b] = its sequence's next position, read on the device."""
+        torch.cat([c.position_dev.expand(b) if c is not None else self._zeros[:b]
                    for c, b in zip(self.caches, self.sizes)], out=self.pos0_branch)
 
     def split_rows(self, rows: torch.Tensor, count: torch.Tensor, bucket: int, N: int):
@@ -435,7 +436,7 @@ class FoldedVerifyEngine:
         buf = self.buffers(B1, N, bucket, P_alloc)
         if causal and self.gate_mode != _lib.SF_GATE_ALL:
             raise ValueError("a causal forward recomputes every row (gate mode SF_GATE_ALL)")
-        self.rope_tables(P + N)
+        self.rope_tables(cache_position(cache) + N)
         if not _device_cache(cache):
             buf.pos0.fill_(P)
         qs = None
@@ -484,14 +485,19 @@ class FoldedVerifyEngine:
     @torch.no_grad()
     def append_blocks(self, tokens: torch.Tensor, cache: PagedKVCache, block: int,
                       causal: bool = False, q_scale: Optional[torch.Tensor] = None,
-                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                      out: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0,
+                      key_mass: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Cache-filling forward of consecutive blocks: tokens [1, n] (n <= CHUNK_ROWS) of
         ``block`` tokens each (the last may be short) through every layer at once, every
         row recomputed, their K/V appended to ``cache`` -> unshifted logits [n, V] (in
         ``out``, [n, V_pad] bf16, if given).  The result of ``forward(..., append=True)``
         block after block -- a row sees the cached keys and its own and earlier blocks'
         (``causal``: itself and earlier rows) -- with the weights read once per
-        CHUNK_ROWS rows instead of once per block.  q_scale: fp32 [n]."""
+        CHUNK_ROWS rows instead of once per block.  q_scale: fp32 [n].
+        ``window`` (> 0): of the keys in front of it a row sees the last window - 1 and the
+        first ``sinks`` only (sf_attn_window).  ``key_mass`` [layers, Hkv, >= cached keys]
+        fp32: what attention every key gets from these rows is added to it
+        (sf_attn_key_mass), which PagedKVCache.evict goes by."""
         n = tokens.shape[1]
         if tokens.shape[0] != 1 or not 1 <= n <= self.CHUNK_ROWS or not 1 <= block <= 64:
             raise ValueError("append_blocks takes [1, n] tokens, n <= "
@@ -506,7 +512,10 @@ class FoldedVerifyEngine:
         buf = self._chunk_bufs.get(cap)
         if buf is None:
             buf = self._chunk_bufs[cap] = _ChunkBuffers(self, cap)
-        cos, sin = self.rope_tables(P + n)
+        cos, sin = self.rope_tables(cache.position + n)
+        bounded = bool(window or sinks) or key_mass is not None
+        if bounded:
+            batch, lse, ws = self._bounded_chunk(cache, n, window, sinks, key_mass)
         if q_scale is not None:
             q_scale = q_scale.reshape(-1).to(device=self.device, dtype=torch.float32).contiguous()
         H, Hkv, hd, D = self.H, self.Hkv, self.hd, self.D
@@ -527,12 +536,20 @@ class FoldedVerifyEngine:
             _lib.qkv_rope_gated(buf.xn, buf.rec, buf.par, 1, n, n, buf.f, buf.src, buf.rows,
                                 buf.count, buf.seg, buf.segcnt, buf.slot, w_qkv, b_qkv, cos, sin,
                                 q_scale, D, H, Hkv, hd, buf.q_buf, buf.kv_buf, buf.ws,
-                                pos0=cache.length_dev)
+                                pos0=cache.position_dev)
             cache.append_rows(li, buf.kv_buf, 0, n)
-            v = cache.view(li)
-            _lib.attn_chunk(buf.q_buf, v.k, v.v, v.page_table, P + n, v.page_size, v.page_stride,
-                            v.head_stride, n, 1 if causal else block, H, Hkv, hd, self.scaling,
-                            buf.o_bf, buf.ws)
+            if bounded:
+                mask = dict(block=1 if causal else block, window=window, sinks=sinks)
+                _lib.attn_window(buf.q_buf, batch, li, H, self.scaling, buf.o_bf, ws, lse=lse,
+                                 **mask)
+                if key_mass is not None:
+                    _lib.attn_key_mass(buf.q_buf, lse, batch, li, H, self.scaling,
+                                       [key_mass[li]], ws, mass_in=[key_mass[li]], **mask)
+            else:
+                v = cache.view(li)
+                _lib.attn_chunk(buf.q_buf, v.k, v.v, v.page_table, P + n, v.page_size,
+                                v.page_stride, v.head_stride, n, 1 if causal else block, H, Hkv,
+                                hd, self.scaling, buf.o_bf, buf.ws)
             _lib.o_proj_post_norm(buf.o_bf, hidden, self._packed_o[li], n, H * hd, D, buf.slot,
                                   lyr.post_attention_layernorm.weight, self.eps, buf.hp, buf.zn,
                                   buf.ws)
@@ -546,24 +563,50 @@ class FoldedVerifyEngine:
         self.last_hidden = last[:n]
         return self.lm_head(buf.final[:n], out=out)
 
+    def _bounded_chunk(self, cache: PagedKVCache, n: int, window: int, sinks: int,
+                       key_mass: Optional[torch.Tensor]):
+        """(batch, lse, workspace) of an append_blocks forward of n rows through
+        sf_attn_window: the workspace is this call's own, sized for its rows and keys."""
+        if window < 0 or sinks < 0 or (sinks and not window):
+            raise ValueError("a window is positive, and sinks go with one")
+        P = cache.length + n
+        need = _lib.attn_window_workspace_bytes(n, self.H)
+        lse = None
+        if key_mass is not None:
+            if key_mass.dim() != 3 or tuple(key_mass.shape[:2]) != (self.L, self.Hkv) or \
+                    key_mass.shape[2] < P or key_mass.dtype != torch.float32:
+                raise ValueError(f"key_mass: expected float32 [{self.L}, {self.Hkv}, >= {P}]")
+            lse = torch.empty(n, self.H, dtype=torch.float32, device=self.device)
+            need = max(need, _lib.attn_key_mass_workspace_bytes(P, self.Hkv))
+        ws = torch.empty(max(need, 256), dtype=torch.uint8, device=self.device)
+        return PagedBatch([cache], [n], ahead=True), lse, ws
+
     @torch.no_grad()
     def append_prompt(self, tokens: torch.Tensor, cache: PagedKVCache, block: int,
-                      causal: bool = False, q_scale=None) -> torch.Tensor:
+                      causal: bool = False, q_scale=None, window: int = 0, sinks: int = 0,
+                      key_mass: Optional[torch.Tensor] = None) -> torch.Tensor:
         """A prompt's blocks appended to ``cache`` -> unshifted logits [1, L, V], as
         ``forward(..., append=True)`` block after block.  Runs of blocks go through
         ``append_blocks``; a single block, and whatever that cannot take (a cache too
         small for the run), one block at a time.  q_scale(P, n): the per-position q scale
-        of n positions from P (fp32 [n] or None), or None."""
+        of n positions from P (fp32 [n] or None), or None.  ``window``, ``sinks``,
+        ``key_mass``: as in append_blocks, which then takes every block."""
         L = tokens.shape[1]
         per = self.CHUNK_ROWS // block * block if 1 <= block <= 64 else 0
         fits = cache.length + L <= min(cache.capacity, self.MAX_KEYS)
-        if not per or L <= block or not fits:
+        bounded = dict(window=window, sinks=sinks, key_mass=key_mass)
+        if window or sinks or key_mass is not None:
+            if not per or not fits:
+                raise ValueError(f"a window or key_mass takes blocks of at most 64 and {L} free "
+                                 f"slots of the cache (capacity {cache.capacity}, at most "
+                                 f"{self.MAX_KEYS} keys)")
+        elif not per or L <= block or not fits:
             prev_mode, self.gate_mode = self.gate_mode, _lib.SF_GATE_ALL
             try:
                 parts = []
                 for s in range(0, L, block):
                     blk = tokens[:, s:s + block]
-                    qs = None if q_scale is None else q_scale(cache.length, blk.shape[1])
+                    qs = None if q_scale is None else q_scale(cache.position, blk.shape[1])
                     parts.append(self.forward(blk, cache, delta=0.0, append=True, q_scale=qs,
                                               causal=causal))
             finally:
@@ -573,8 +616,9 @@ class FoldedVerifyEngine:
         for s in range(0, L, per):
             blk = tokens[:, s:s + per]
             n = blk.shape[1]
-            qs = None if q_scale is None else q_scale(cache.length, n)
-            self.append_blocks(blk, cache, block, causal=causal, q_scale=qs, out=logits[s:s + n])
+            qs = None if q_scale is None else q_scale(cache.position, n)
+            self.append_blocks(blk, cache, block, causal=causal, q_scale=qs, out=logits[s:s + n],
+                               **bounded)
         # as after a forward of the last block alone
         last = (n - 1) // block * block
         self.last_hidden = self.last_hidden[last:]
@@ -642,7 +686,7 @@ class FoldedVerifyEngine:
         bucket = BN if bucket is None else max(1, min(int(bucket), BN))
         P_alloc = max([c.capacity for c in caches if c is not None], default=0)
         buf = self.buffers(B1, N, bucket, P_alloc)
-        self.rope_tables(max(cache_length(c) for c in caches) + N)
+        self.rope_tables(max(cache_position(c) for c in caches) + N)
         q_scaled = q_scales is not None and any(q is not None for q in q_scales)
         if self.use_graphs and trace is None:
             hidden = self._replay_batched(buf, tokens, sizes, caches, N, delta, bucket,
@@ -734,7 +778,7 @@ class FoldedVerifyEngine:
             batch.refresh_positions()
         hidden = base.embed_tokens(tokens).reshape(BN, D)
         cos, sin = self._rope
-        pos0 = cache.length_dev if _device_cache(cache) else buf.pos0
+        pos0 = cache.position_dev if _device_cache(cache) else buf.pos0
         for li, lyr in enumerate(self.layers):
             count = buf.count_slab[li:li + 1]
             segcnt = buf.segcnt_slab[li * B1:(li + 1) * B1]
@@ -858,8 +902,10 @@ class FoldedVerifyEngine:
         if isinstance(cache, ContiguousMirror):
             return (id(cache), cache.k.data_ptr(), cache.v.data_ptr(),
                     cache.length_dev.data_ptr(), cache.capacity)
+        # (position_dev: a buffer of its own once keys were evicted)
         return (id(cache), cache.k_pages.data_ptr(), cache.v_pages.data_ptr(),
-                cache.page_table.data_ptr(), cache.length_dev.data_ptr(), cache.capacity)
+                cache.page_table.data_ptr(), cache.length_dev.data_ptr(),
+                cache.position_dev.data_ptr(), cache.capacity)
 
     def invalidate_prefix(self) -> None:
         """Make the next step re-read a reference-style cache in full (after the
@@ -984,7 +1030,7 @@ class FoldedVerifyEngine:
                                     segcnt, buf.slot, buf.rstd, buf.xn)
 
         cos, sin = self._rope
-        pos0 = cache.length_dev if _device_cache(cache) else buf.pos0
+        pos0 = cache.position_dev if _device_cache(cache) else buf.pos0
 
         def qkv():
             if self.gated_qkv:

@@ -22,7 +22,7 @@ from typing import Callable, Dict, List, Optional, Sequence
 import torch
 
 from specfold_amd.engine import StepStats
-from specfold_amd.kv_cache import cache_length
+from specfold_amd.kv_cache import cache_position
 
 # [(batched [B1_s, N], prefix cache)] -> [logits [B1_s, N, V]]
 ForwardMany = Callable[[List[tuple]], List[torch.Tensor]]
@@ -72,7 +72,7 @@ class LockstepDecoder:
         N = requests[0][0].shape[1]
         total = sum(b.shape[0] for b, _ in requests) * N      # real (unpadded) rows
         q_scale = getattr(g0.model_executor, "q_scale", None)
-        q_scales = [q_scale(cache_length(c), N) if q_scale is not None else None
+        q_scales = [q_scale(cache_position(c), N) if q_scale is not None else None
                     for _, c in requests]
         # a batched step holds at most 64 branches and 1024 rows: split the round
         # into as few steps as fit

@@ -24,7 +24,7 @@ from specfold_amd import _lib
 from specfold_amd.engine import FoldedVerifyEngine, StepStats, build_parent_map
 from specfold_amd.generate.nld_generation import NLDDiffusionGeneration
 from specfold_amd.generate.nld_model_executor import llama4_q_scale
-from specfold_amd.kv_cache import cache_length
+from specfold_amd.kv_cache import cache_position
 
 logger = logging.getLogger(__name__)
 
@@ -80,7 +80,7 @@ class SpecFoldHIPNLDGeneration(NLDDiffusionGeneration):
             self._pack_layer_weights()
         eng = self._engine
         N = self.block_length
-        q_scale = llama4_q_scale(self.model_executor.model.config, cache_length(cache), N,
+        q_scale = llama4_q_scale(self.model_executor.model.config, cache_position(cache), N,
                                  eng.device)
         main = torch.full((1, N), self.mask_id, dtype=torch.long, device=eng.device)
         NLDDiffusionGeneration._batched_block_forward(self, main, cache)
@@ -107,7 +107,7 @@ class SpecFoldHIPNLDGeneration(NLDDiffusionGeneration):
             self._pack_layer_weights()
         eng = self._engine
         bucket = B1 * N if self.fold_bucket is None else min(self.fold_bucket, B1 * N)
-        q_scale = llama4_q_scale(self.model_executor.model.config, cache_length(past_key_values),
+        q_scale = llama4_q_scale(self.model_executor.model.config, cache_position(past_key_values),
                                  N, eng.device)
         stats = StepStats()
         prev_mode, eng.gate_mode = eng.gate_mode, self.gate_mode

@@ -30,7 +30,7 @@ import torch
 from specfold_amd import _lib
 from specfold_amd.engine import FoldedVerifyEngine
 from specfold_amd.generate.fastdllm_model_executor import ByteTokenizer
-from specfold_amd.kv_cache import PagedKVCache, cache_length
+from specfold_amd.kv_cache import PagedKVCache, cache_position
 
 
 def llama4_q_scale(config, P: int, N: int, device=None) -> Optional[torch.Tensor]:
@@ -122,7 +122,7 @@ class NLDModelExecutor:
                 logits = eng.append_prompt(input_seq, cache, self.block_length, causal=causal,
                                            q_scale=self.q_scale)
                 return SimpleNamespace(logits=logits, past_key_values=cache)
-            qs = self.q_scale(cache_length(past_key_values), input_seq.shape[1])
+            qs = self.q_scale(cache_position(past_key_values), input_seq.shape[1])
             logits = eng.forward(input_seq, past_key_values, delta=0.0, q_scale=qs, causal=causal)
             return SimpleNamespace(logits=logits, past_key_values=past_key_values)
         finally:

@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import weakref
 from dataclasses import dataclass
-from typing import List, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -64,6 +64,26 @@ class PagedKVCache:
         self.length = 0
         # device copy of the length, read by the attention kernel (graph-stable)
         self.length_dev = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.evicted = 0            # keys dropped by evict
+        self._position_dev: Optional[torch.Tensor] = None
+
+    # -- positions: the next token's, which an evicted cache's length falls behind ------
+    @property
+    def position(self) -> int:
+        return self.length + self.evicted
+
+    @property
+    def position_dev(self) -> torch.Tensor:
+        """Device int32[1] copy of ``position`` (length_dev itself until keys are evicted)."""
+        return self.length_dev if self._position_dev is None else self._position_dev
+
+    def _set_length(self, length: int, evicted: int) -> None:
+        self.length, self.evicted = length, evicted
+        self.length_dev.fill_(length)
+        if evicted and self._position_dev is None:
+            self._position_dev = torch.empty_like(self.length_dev)
+        if self._position_dev is not None:
+            self._position_dev.fill_(length + evicted)
 
     # -- the reference cache contract ------------------------------------------------
     def get_seq_length(self, layer_idx: int = 0) -> int:
@@ -105,8 +125,36 @@ class PagedKVCache:
     def advance(self, n_tok: int) -> None:
         if self.length + n_tok > self.capacity:
             raise ValueError("KV cache full")
-        self.length += n_tok
-        self.length_dev.fill_(self.length)
+        self._set_length(self.length + n_tok, self.evicted)
+
+    def evict(self, key_mass: torch.Tensor, keep: int, sinks: int = 0, recent: int = 0,
+              into: Optional["PagedKVCache"] = None, kept: Optional[torch.Tensor] = None,
+              mass_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Keep ``keep`` of the cached keys of every layer and kv head: the first ``sinks``,
+        the last ``recent`` and, of the others, those with the largest ``key_mass``
+        [layers, Hkv, >= length] fp32 (equal: the lower slot; NaN above every number), in
+        their order.  In place, ``key_mass`` moving with them (its entries keep .. length - 1
+        are zeroed; or to ``mass_out``); or into the cache ``into`` (same layers and heads;
+        what it held goes), which leaves this one and ``key_mass`` as they are (``mass_out``
+        [layers, Hkv, >= keep]: the kept keys' mass).  Returns the kept keys' old slots
+        [layers, Hkv, keep] int32 (``kept`` if given).  The keys keep their RoPE angles:
+        ``position`` goes on where it was, ``length`` is ``keep``."""
+        if not 1 <= keep <= self.length:
+            raise ValueError(f"keep must be in [1, {self.length}], got {keep}")
+        if sinks < 0 or recent < 0 or sinks + recent > keep:
+            raise ValueError(f"sinks {sinks} + recent {recent} must fit in keep {keep}")
+        dst = self if into is None else into
+        if into is self:
+            raise ValueError("into is this cache: leave it out to evict in place")
+        if into is None and mass_out is None:
+            mass_out = key_mass
+        if kept is None:
+            kept = torch.empty(self.num_layers, self.Hkv, keep, dtype=torch.int32,
+                               device=self.device)
+        _lib.kv_evict(key_mass, self.length, keep, sinks, recent, self, dst, kept,
+                      mass_out=mass_out)
+        dst._set_length(keep, self.position - keep)
+        return kept
 
     def load_dense(self, kv: Sequence[Tuple[torch.Tensor, torch.Tensor]]) -> None:
         """Fill from per-layer ([1, Hkv, P, hd], [1, Hkv, P, hd]) tensors (any device)."""
@@ -124,8 +172,57 @@ class PagedKVCache:
                     x = torch.cat([x, x.new_zeros(self.Hkv, pad, self.hd)], dim=1)
                 x = x.reshape(self.Hkv, npg, ps, self.hd).permute(1, 0, 2, 3)
                 dst[li].index_copy_(0, idx, x.contiguous())
-        self.length = P
-        self.length_dev.fill_(P)
+        self._set_length(P, 0)
+
+
+class PagedBatch:
+    """New rows of several sequences over their caches, as sf_attn_window and
+    sf_attn_key_mass take them: ``rows[s]`` rows of sequence s (0 allowed), packed one
+    sequence behind the other, whose K/V are the last keys of ``caches[s]`` (PagedKVCache
+    or ContiguousMirror; alike in kv heads, head size and page size).  Lengths are read
+    from the caches at every call.  ``ahead``: the rows are appended (append_rows) but not
+    yet counted (advance)."""
+
+    def __init__(self, caches: Sequence, rows: Sequence[int], ahead: bool = False):
+        if not caches or len(caches) != len(rows):
+            raise ValueError("a batch needs one row count per cache")
+        c0 = caches[0]
+        paged = [c for c in caches if isinstance(c, PagedKVCache)]
+        self.Hkv, self.hd = c0.Hkv, c0.hd
+        self.page_size = paged[0].page_size if paged else 16
+        self.caches, self.rows, self.ahead = list(caches), [int(n) for n in rows], ahead
+        self.num_rows = sum(self.rows)
+        self.device = c0.length_dev.device
+        for c, n in zip(self.caches, self.rows):
+            if not isinstance(c, (PagedKVCache, ContiguousMirror)):
+                raise TypeError("a batch takes PagedKVCache or ContiguousMirror caches")
+            if c.Hkv != self.Hkv or c.length_dev.device != self.device or \
+                    (isinstance(c, PagedKVCache) and c.page_size != self.page_size):
+                raise ValueError("the caches of a batch share kv heads, page size and device")
+            if n < 0:
+                raise ValueError("a row count must not be negative")
+        self._layers: Dict[int, object] = {}
+
+    def seqs(self, li: int):
+        """Layer li's sf_kv_seq array at the caches' present lengths."""
+        arr, arr_views = self._layers.get(li, (None, []))
+        if arr is None:
+            arr = (_lib.KVSeq * len(self.caches))()
+            for s, c in zip(arr, self.caches):
+                vw = c.view(li)
+                _lib._need(vw.k, "k", torch.bfloat16)
+                _lib._need(vw.v, "v", torch.bfloat16)
+                s.k, s.v = vw.k.data_ptr(), vw.v.data_ptr()
+                s.page_table = None if vw.page_table is None else vw.page_table.data_ptr()
+                s.page_stride, s.head_stride = vw.page_stride, vw.head_stride
+                s.pages = 0 if vw.page_table is None else vw.k.shape[0]
+                arr_views.append(vw)
+            self._layers[li] = arr, arr_views    # (the views keep the buffers)
+        for s, c, n in zip(arr, self.caches, self.rows):
+            s.length, s.rows = c.length + (n if self.ahead else 0), n
+            if s.length > c.capacity:
+                raise ValueError(f"{s.length} keys exceed the cache's capacity {c.capacity}")
+        return arr
 
 
 class ContiguousMirror:
@@ -159,6 +256,10 @@ class ContiguousMirror:
         self.length_dev = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._sig = None
         self._refs: tuple = ()
+
+    @property
+    def position_dev(self) -> torch.Tensor:
+        return self.length_dev
 
     def get_seq_length(self, layer_idx: int = 0) -> int:
         return self.length
@@ -244,6 +345,11 @@ def cache_length(cache) -> int:
     if len(cache) == 0 or cache[0][0] is None:
         return 0
     return int(cache[0][0].shape[-2])
+
+
+def cache_position(cache) -> int:
+    """Absolute position of the next token: the prefix length and what was evicted of it."""
+    return cache.position if isinstance(cache, PagedKVCache) else cache_length(cache)
 
 
 def _weakrefable(obj) -> bool:

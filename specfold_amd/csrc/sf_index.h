@@ -519,6 +519,54 @@ inline int prefix_launch_grid(int qmax, int nch, int Hkv) {
 }  // namespace sfa
 
 // ---------------------------------------------------------------------------
+// Attention with window and sinks (sf_window.hip)
+// ---------------------------------------------------------------------------
+namespace sfw {
+
+constexpr int kStage = 32;   // keys of an LDS stage
+
+// Row m of n rows over P cached keys (its position p = P - n + m) sees the keys below
+// row_end that are below `sinks` or not below row_lo.
+SF_IDX int row_end(int m, int n, int P, int block) {
+  const long long e = ((long long)(m / block) + 1) * block;
+  return P - n + (int)(e < n ? e : n);
+}
+SF_IDX int row_lo(int m, int n, int P, int window) {
+  const int p = P - n + m;
+  return window > 0 && p >= window ? p - window + 1 : 0;
+}
+
+// The key stages that rows [m0, m1] see between them: stages [0, sink_st), then
+// [lo_st, lo_st + nst - sink_st); the i-th of the nst stages starts at key key0(i).
+struct Keys {
+  int sink_st, lo_st, nst;
+  SF_IDX int stage(int i) const { return i < sink_st ? i : lo_st + i - sink_st; }
+  SF_IDX int key0(int i) const { return stage(i) * kStage; }
+};
+SF_IDX Keys tile_keys(int m0, int m1, int n, int P, int block, int window, int sinks) {
+  const int st_end = (row_end(m1, n, P, block) + kStage - 1) / kStage;
+  const int lo = row_lo(m0, n, P, window);
+  int lo_st = lo / kStage;
+  int sink_st = (sf_imin(sinks, lo) + kStage - 1) / kStage;
+  if (sink_st >= lo_st) sink_st = lo_st = 0;
+  return Keys{sink_st, lo_st, sink_st + st_end - lo_st};
+}
+
+// Queries of a sequence and kv head are its rows x the G heads, qi = m * G + g, cut into
+// tiles of bq; a tile's stages are cut into ranges of spr.
+SF_IDX int tiles_of(int rows, int G, int bq) { return (rows * G + bq - 1) / bq; }
+SF_IDX Keys query_tile_keys(int t, int bq, int G, int n, int P, int block, int window, int sinks) {
+  const int q1 = sf_imin(n * G, (t + 1) * bq) - 1;
+  return tile_keys(t * bq / G, q1 / G, n, P, block, window, sinks);
+}
+
+// Ranges a query's keys are cut into at most, by the rows of the call (bounds the
+// workspace of partial sums: 4096 row partials, or 4 of every row).
+SF_IDX int ranges_cap(int rows) { return rows >= 1024 ? 4 : (rows <= 64 ? 64 : 4096 / rows); }
+
+}  // namespace sfw
+
+// ---------------------------------------------------------------------------
 // Greedy statistics (sf_logits.hip): the slices of a logits row
 // ---------------------------------------------------------------------------
 namespace sfl {

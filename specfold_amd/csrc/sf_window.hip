@@ -6,110 +6,790 @@
 // p = P - n + m and sees the keys t < end(m) = P - n + min(n, (m / block + 1) * block)
 // with t < sinks or t > p - window (window 0: all).  o = softmax(scaling q.k) v,
 // lse = ln sum exp(scaling q.k); mass[t] += exp(scaling q.k - lse).
+//
+// Attention.  The queries of a (sequence, kv head) are its rows x the G q-heads, qi =
+// m * G + g, cut into tiles; a tile walks the 32-key stages that its rows see, running
+// maximum and sum per query, and skips the stages between the sinks and the window.
+// Scores are formed transposed, S^T = K Q^T (v_mfma_f32_32x32x16_bf16, K the A operand),
+// so a lane holds 16 of a stage's keys for ONE query (lane % 32) and the softmax is in
+// the lane; registers 8kk .. 8kk + 7 of S^T are the B operand of O^T += V^T P^T for the
+// keys 16kk + {8 (e / 4) + 4 (lane / 32) + e % 4} without a shuffle, and V^T comes in
+// the same key order from row-major V by transposing LDS reads.
 #include <math.h>
 
 #include "sf_common.h"
+#include "sf_index.h"
 
 namespace {
+
+using namespace sfw;
 
 constexpr int kHD = 128;
 constexpr int kMaxSeqs = 32;
 constexpr int kMaxKeys = 32768;
 constexpr int kMaxG = 16;
+constexpr int kThreads = 256;
+constexpr int kCUs = 256;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kLazy = 8.f;   // base-2 headroom of the softmax reference
+
+typedef float sf_f32x16 __attribute__((ext_vector_type(16)));
+
+SF_DEV sf_f32x16 mfma32(const sf_bf16x8 a, const sf_bf16x8 b, const sf_f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+
+// Lane i's value of v (i wave-uniform), and a wait for all but the N youngest vector
+// memory operations of this wave without a workgroup barrier (the wave's lanes are
+// through with what they did before).  Elsewhere than on the GPU the wave's lanes are
+// only kept in step.
+#if defined(__HIPCC__)
+SF_DEV int lane_value(int v, int i) { return __builtin_amdgcn_readlane(v, i); }
+template <int N>
+SF_DEV void wait_vm_wave() {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));   // lgkmcnt(0) too
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+#else
+inline int lane_value(int v, int i) { return __shfl(v, i, 64); }
+template <int N>
+inline void wait_vm_wave() { (void)__builtin_amdgcn_readfirstlane(0); }
+#endif
 
 struct Seq {
   const uint16_t* k;
   const uint16_t* v;
   const int32_t* table;
-  const float* mass_in;
-  float* mass_out;
-  long long page_stride, head_stride, mass_in_stride, mass_out_stride;
+  long long page_stride, head_stride;
   int length, rows, row0, pages;
+  int tile0, tiles;        // of the launch this sequence belongs to (0 tiles: of another)
 };
 struct Call {
   Seq s[kMaxSeqs];
-  int n_seqs, page_size, block, window, sinks, H, Hkv, rows;
+  int n_seqs, page_shift, block, window, sinks, H, Hkv, rows;
+  int tiles, nr, spr;      // tiles of all sequences, ranges of a tile, stages of a range
 };
 
-SF_DEV long long key_off(const Seq& s, int page_size, int h, int t) {
-  long long off = (long long)h * s.head_stride;
-  if (!s.table) return off + (long long)t * kHD;
-  const int lp = t / page_size;
-  const int id = s.table[lp];
-  return off + (id >= 0 && id < s.pages ? id : 0) * s.page_stride +
-         (long long)(t - lp * page_size) * kHD;
-}
-SF_DEV int row_end(const Call& c, const Seq& s, int m) {
-  const long long e = ((long long)(m / c.block) + 1) * c.block;
-  return s.length - s.rows + (int)(e < s.rows ? e : s.rows);
-}
-SF_DEV int row_lo(const Call& c, const Seq& s, int m) {
-  const int p = s.length - s.rows + m;
-  return c.window && p >= c.window ? p - c.window + 1 : 0;
+SF_DEV int page_of(const Seq& s, int page_shift, int key) {
+  const int id = s.table[key >> page_shift];
+  return id >= 0 && id < s.pages ? id : 0;
 }
 
-// One wave per (row, q-head), 64 keys at a time: a key per lane for the scores, two dims
-// per lane for the values.
-__global__ __launch_bounds__(256) void sf_window_attn_kernel(const uint16_t* __restrict__ q,
-                                                             Call c, float scaling,
-                                                             uint16_t* __restrict__ o,
-                                                             float* __restrict__ lse) {
+// ---- LDS stages ------------------------------------------------------------------------
+// 32 keys: K rows of 256 bytes, then V rows; 16-byte unit u of row r at unit u ^ (r & 15)
+// (K: the 16-row operand reads hit 16 different units) and u ^ 2 (r & 7) (V: the
+// transposing reads take four consecutive rows x 64 bytes).
+constexpr int kRowBytes = 2 * kHD;
+constexpr int kHalf = kStage * kRowBytes;    // K rows of a stage
+constexpr int kSlot = 2 * kHalf;             // 16 KB
+
+// This lane's byte offsets in a slot: K operand (key lane % 32, dims 16ks + 8 (lane / 32)
+// .. + 8) and V^T operand of dim tile dt (32 dims, keys 4 (lane / 32) + {0..3}; the next
+// 8 keys 8 rows on).
+SF_DEV uint32_t k_off(int lane, int ks) {
+  const int r = lane & 31, u = 2 * ks + (lane >> 5);
+  return (uint32_t)(r * kRowBytes + (u ^ (r & 15)) * 16);
+}
+SF_DEV uint32_t v_off(int lane, int dt) {
+  const int r = 4 * (lane >> 5) + ((lane & 15) >> 2);
+  const int u = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  return (uint32_t)(kHalf + r * kRowBytes + (u ^ (2 * (r & 7))) * 16 + (lane & 1) * 8);
+}
+
+// Copies rows row0 .. + 4 N of the 16-key group that starts at key g0 to a stage, `dst`
+// the group's first row there: keys behind the last repeat it.  page: the group's page.
+template <int N>
+SF_DEV void copy_rows(const uint16_t* base, const Seq& s, int page_shift, int page, int g0,
+                      int row0, const int (&unit_off)[N], uint8_t* dst) {
+  const int lane = threadIdx.x & 63;
+  const uint16_t* src = base + (s.table ? (long long)page * s.page_stride +
+                                              (long long)(g0 & ((1 << page_shift) - 1)) * kHD
+                                        : (long long)g0 * kHD);
+  const int last = s.length - 1 - g0;
+  if (last >= 15) {   // wave-uniform
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      sf_lds_dma16(src + (row0 + 4 * i + (lane >> 4)) * kHD + unit_off[i],
+                   dst + (row0 + 4 * i) * kRowBytes);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      sf_lds_dma16(src + min(row0 + 4 * i + (lane >> 4), last) * kHD + unit_off[i],
+                   dst + (row0 + 4 * i) * kRowBytes);
+  }
+}
+// the logical unit (in elements) that this lane's copy of rows r0 .. + 4 brings
+SF_DEV int copy_unit(int lane, int r0, bool is_v) {
+  const int r = r0 + (lane >> 4), p = lane & 15;
+  return (is_v ? p ^ (2 * (r & 7)) : p ^ (r & 15)) * 8;
+}
+
+SF_DEV int last_group(int P) { return (P - 1) & ~15; }
+
+// p[.] of one query of a stage (16 keys a lane) -> the two B operands
+SF_DEV void pack_p(const float (&p)[16], sf_u32x4 (&pb)[2]) {
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) pb[kk][w] = sf_pack2(p[8 * kk + 2 * w], p[8 * kk + 2 * w + 1]);
+}
+
+// The mask of a stage's scores for one query: keys at or behind `end`, and keys of
+// [sinks, lo).
+SF_DEV void mask_scores(sf_f32x16& s, int key0, int hf, int end, int lo, int sinks) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int key = key0 + 8 * (i >> 2) + 4 * hf + (i & 3);
+    if (key >= end || (key < lo && key >= sinks)) s[i] = -INFINITY;
+  }
+}
+
+// Queries q0 .. q0 + nw of an item a key at a time, for a wave whose masked stages held a
+// value that is not finite: the weight of a hidden key is 0, but 0 * inf is not.  Lane: a
+// key of 64 for the scores, two dims for the values.  One range is written to o and lse,
+// of several the partial.
+struct Out {
+  uint16_t* o;
+  float* lse;
+  float* ws_o;
+  float* ws_ml;
+  float scale_log2;
+};
+SF_DEV void slow_queries(const uint16_t* q, const Call& c,
+                                                       const Seq& s, int h, int r, int q0, int nw,
+                                                       Keys keys, int c0, int nst, const Out& out) {
+  const int lane = threadIdx.x & 63, G = c.H / c.Hkv;
+  const long long head = (long long)h * s.head_stride;
+  auto key_at = [&](int t) {
+    return head + (s.table ? page_of(s, c.page_shift, t) * s.page_stride +
+                                 (long long)(t & ((1 << c.page_shift) - 1)) * kHD
+                           : (long long)t * kHD);
+  };
+  for (int qi = q0; qi < min(q0 + nw, s.rows * G); ++qi) {
+    const int m = qi / G;
+    const int end = row_end(m, s.rows, s.length, c.block);
+    const int lo = row_lo(m, s.rows, s.length, c.window);
+    const size_t rh = (size_t)(s.row0 + m) * c.H + h * G + (qi - m * G);
+    float mx = -INFINITY, l = 0.f, a0 = 0.f, a1 = 0.f;
+    for (int k = 0; k < nst; k += 2) {   // two stages: 64 keys
+      const int kk = k + (lane >> 5);
+      const int t = keys.key0(c0 + min(kk, nst - 1)) + (lane & 31);
+      const bool see = kk < nst && t < end && (t < c.sinks || t >= lo);
+      float x = -INFINITY;
+      if (see) {
+        const uint16_t* kr = s.k + key_at(t);
+        x = 0.f;
+        for (int d = 0; d < kHD; d += 8) {
+          float a[8], b[8];
+          sf_unpack8(*reinterpret_cast<const sf_u32x4*>(kr + d), a);
+          sf_unpack8(*reinterpret_cast<const sf_u32x4*>(q + rh * kHD + d), b);
+          for (int i = 0; i < 8; ++i) x = fmaf(a[i], b[i], x);
+        }
+        x *= out.scale_log2;
+      }
+      const float nm = fmaxf(mx, sf_wave_max(x));
+      const float mu = nm == -INFINITY ? 0.f : nm;
+      const float alpha = __builtin_amdgcn_exp2f(mx - mu);
+      const float p = see ? __builtin_amdgcn_exp2f(x - mu) : 0.f;
+      l = l * alpha + sf_wave_sum(p);
+      a0 *= alpha;
+      a1 *= alpha;
+      mx = nm;
+      for (unsigned long long bits = __ballot(see); bits; bits &= bits - 1) {
+        const int j = __builtin_ctzll(bits);
+        const float pj = __shfl(p, j, 64);
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(
+            s.v + key_at(keys.key0(c0 + k + (j >> 5)) + (j & 31)) + 2 * lane);
+        a0 = fmaf(pj, __uint_as_float(w << 16), a0);
+        a1 = fmaf(pj, __uint_as_float(w & 0xffff0000u), a1);
+      }
+    }
+    if (c.nr == 1) {
+      *reinterpret_cast<uint32_t*>(out.o + rh * kHD + 2 * lane) = sf_pack2(a0 / l, a1 / l);
+      if (out.lse && lane == 0) out.lse[rh] = mx * kLn2 + logf(l);
+    } else {
+      const size_t slot = (size_t)r * c.rows * c.H + rh;
+      out.ws_o[slot * kHD + 2 * lane] = a0;
+      out.ws_o[slot * kHD + 2 * lane + 1] = a1;
+      if (lane == 0) out.ws_ml[2 * slot] = mx, out.ws_ml[2 * slot + 1] = l;
+    }
+  }
+}
+
+// Whether any of the wave's V^T operands has an exponent of all ones.
+SF_DEV bool any_not_finite(const sf_u32x2 (&vf)[16]) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    t |= ((vf[i][0] & 0x7f807f80u) + 0x00800080u) | ((vf[i][1] & 0x7f807f80u) + 0x00800080u);
+  return __ballot((t & 0x80008000u) != 0) != 0;
+}
+
+// The V^T operands of a stage (dim tile dt, 16 keys kk, 8-key halves): vf[8kk + 2dt + r].
+template <int OFF>
+SF_DEV void read_v(const sf_lds_off (&va)[4], sf_u32x2 (&vf)[16]) {
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) {
+    vf[2 * dt] = sf_lds_read8_tr<OFF>(va[dt]);
+    vf[2 * dt + 1] = sf_lds_read8_tr<OFF + 8 * kRowBytes>(va[dt]);
+    vf[8 + 2 * dt] = sf_lds_read8_tr<OFF + 16 * kRowBytes>(va[dt]);
+    vf[8 + 2 * dt + 1] = sf_lds_read8_tr<OFF + 24 * kRowBytes>(va[dt]);
+  }
+}
+template <int OFF>
+SF_DEV void read_k(const sf_lds_off (&ka)[8], sf_u32x4 (&kf)[8]) {
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) kf[ks] = sf_lds_read16<OFF>(ka[ks]);
+}
+SF_DEV sf_bf16x8 v_operand(const sf_u32x2 (&vf)[16], int kk, int dt) {
+  const sf_u32x2 a = vf[8 * kk + 2 * dt], b = vf[8 * kk + 2 * dt + 1];
+  return sf_as_bf16x8(sf_u32x4{a[0], a[1], b[0], b[1]});
+}
+
+// One query's result: unnormalised o (registers 16dt' ..), reference m (base 2) and sum l.
+SF_DEV void write_direct(const sf_f32x16 (&acc)[4], float m, float l, int hf, uint16_t* o,
+                         float* lse) {
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      sf_u32x2 w;
+      w[0] = sf_pack2(acc[dt][4 * b] * inv, acc[dt][4 * b + 1] * inv);
+      w[1] = sf_pack2(acc[dt][4 * b + 2] * inv, acc[dt][4 * b + 3] * inv);
+      *reinterpret_cast<sf_u32x2*>(o + 32 * dt + 8 * b + 4 * hf) = w;
+    }
+  if (lse && hf == 0) *lse = m * kLn2 + logf(l);
+}
+SF_DEV void write_partial(const sf_f32x16 (&acc)[4], float m, float l, int hf, float* po,
+                          float* pml) {
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      sf_handoff_store(reinterpret_cast<sf_f32x4*>(po + 32 * dt + 8 * b + 4 * hf),
+                       sf_f32x4{acc[dt][4 * b], acc[dt][4 * b + 1], acc[dt][4 * b + 2],
+                                acc[dt][4 * b + 3]});
+  if (hf == 0) sf_handoff_store(reinterpret_cast<sf_f32x2*>(pml), sf_f32x2{m, l});
+}
+
+// Work item of block b: the kv head fastest (blocks go round robin over the 8 XCDs, so
+// with 1, 2, 4 or 8 kv heads a head stays on its XCDs and their L2), then the range, then
+// the sequences' tiles, the last tile of a sequence (the most keys) first.
+struct Item {
+  int si, tile, r, h;
+};
+SF_DEV Item find_item(const Call& c) {
+  Item it;
+  it.h = blockIdx.x % c.Hkv;
+  const int rest = blockIdx.x / c.Hkv;
+  it.r = rest % c.nr;
+  const int tt = rest / c.nr;
+  it.si = 0;
+  while (tt >= c.s[it.si].tile0 + c.s[it.si].tiles) ++it.si;
+  it.tile = c.s[it.si].tiles - 1 - (tt - c.s[it.si].tile0);
+  return it;
+}
+
+// ---- tiles of 32 W queries -----------------------------------------------------------------
+// W waves, two on each SIMD (W = 8: one workgroup a CU, W = 4: two), wave w the queries
+// 32 w .. + 32 of the tile, all walking the same stages through an LDS ring that direct
+// copies fill kAhead stages ahead.  The step of stage k runs three independent things
+// side by side within the wave, the matrix core's and the vector ALU's: the softmax of
+// stage k, O^T += V^T P^T of stage k - 1 and S^T of stage k + 1.
+template <int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
+                      uint16_t* __restrict__ o, float* __restrict__ lse, float* __restrict__ ws_o,
+                      float* __restrict__ ws_ml) {
+  constexpr int kRing = W;
+  constexpr int kAhead = kRing - 1;
+  constexpr int kCopies = 16 / W;   // of a wave per stage: 4 rows each
+  __shared__ __attribute__((aligned(16))) uint8_t ring[kRing * kSlot];
+  __shared__ int s_pg[2 * (kMaxKeys / kStage) + 64];
+  const Item it = find_item(c);
+  const Seq& s = c.s[it.si];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, hf = lane >> 5;
+  const int G = c.H / c.Hkv, nq = s.rows * G, P = s.length;
+  constexpr int kBQ = 32 * W;
+  const Keys keys = query_tile_keys(it.tile, kBQ, G, s.rows, P, c.block, c.window, c.sinks);
+  const int c0 = it.r * c.spr;
+  if (c0 >= keys.nst) return;
+  const int nst = min(c.spr, keys.nst - c0);
+  const int lastg = last_group(P);
+
+  // the page of every 16-key group of the range; the queries
+  if (s.table)
+    for (int i = tid; i < 2 * nst; i += 64 * W)
+      s_pg[i] = page_of(s, c.page_shift, min(keys.key0(c0 + (i >> 1)) + 16 * (i & 1), lastg));
+  const int q0 = it.tile * kBQ + wv * 32;   // the wave's first query
+  const int qi = min(q0 + (lane & 31), nq - 1);   // padding: the last query again
+  const int m = qi / G;
+  const int end = row_end(m, s.rows, P, c.block), lo = row_lo(m, s.rows, P, c.window);
+  const size_t rh = (size_t)(s.row0 + m) * c.H + it.h * G + (qi - m * G);
+  sf_u32x4 qf[8];
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks)
+    qf[ks] = *reinterpret_cast<const sf_u32x4*>(q + rh * kHD + 8 * hf + 16 * ks);
+  // stages whose keys every query of the wave sees need no mask
+  const int end_min = row_end(min(q0, nq - 1) / G, s.rows, P, c.block);
+  const int lo_max = row_lo(min(q0 + 31, nq - 1) / G, s.rows, P, c.window);
+  sf_wait_vm_loads();
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) sf_pin(qf[ks]);
+  __syncthreads();   // s_pg
+
+  // copies: 16-key group wv * 4 / W of K0, K1, V0, V1
+  const int part = wv * 4 / W, grp = part & 1;
+  const bool is_v = part >= 2;
+  const int row0 = W == 8 ? 8 * (wv & 1) : 0;   // of the group
+  const uint16_t* base = (is_v ? s.v : s.k) + (long long)it.h * s.head_stride;
+  int unit_off[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) unit_off[i] = copy_unit(lane, row0 + 4 * i, is_v);
+  const sf_lds_off pg_addr = sf_lds_addr(s_pg) + 4 * lane;
+  int pg = 0;   // lane i: the page of group i of the 32 stages being copied
+  auto issue = [&](int k) {
+    const int kc = min(k, nst - 1);   // past the range: its last stage again
+    if (s.table && (k & 31) == 0) pg = (int)sf_lds_read4_now(pg_addr + 4 * 64 * (kc >> 5));
+    const int g0 = min(keys.key0(c0 + kc) + 16 * grp, lastg);
+    const int page = s.table ? lane_value(pg, 2 * (kc & 31) + grp) : 0;
+    copy_rows<kCopies>(base, s, c.page_shift, page, g0, row0, unit_off,
+                       ring + (k % kRing) * kSlot + (is_v ? kHalf : 0) + 16 * grp * kRowBytes);
+  };
+#pragma unroll 1
+  for (int k = 0; k < kAhead; ++k) issue(k);
+
+  uint32_t koff[8], voff[4];
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) koff[ks] = k_off(lane, ks);
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) voff[dt] = v_off(lane, dt);
+
+  // online softmax per query: acc and l_run are kept against the reference m_ref (-inf:
+  // nothing yet), which moves up to the running maximum m_hi only when a score passes it
+  // by more than kLazy; m_hi and l_run are per lane (its own keys).
+  float m_ref = -INFINITY, m_hi = -INFINITY, l_run = 0.f, alpha = 1.f;
+  sf_f32x16 acc[4], sa, sb;
+  sf_u32x2 vf[16];
+  sf_u32x4 pa[2], pb[2];
+  bool resc = false, bad = false;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
+  pb[0] = pb[1] = sf_u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) vf[i] = sf_u32x2{0u, 0u};
+
+  auto qk = [&](const sf_u32x4 (&kf)[8], sf_f32x16& out) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) out[i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) out = mfma32(sf_as_bf16x8(kf[ks]), sf_as_bf16x8(qf[ks]), out);
+  };
+
+  // S^T of stage 0
+  sf_wait_vm_barrier<(kAhead - 1) * kCopies>();
+  {
+    sf_lds_off ka[8];
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) ka[ks] = sf_lds_addr(ring) + koff[ks];
+    sf_u32x4 kf[8];
+    read_k<0>(ka, kf);
+    sf_lds_reads_done(kf);
+    qk(kf, sa);
+  }
+
+  // stage k: its scores in sc, its P^T to pc; stage k - 1's V^T in vf and P^T in pp; stage
+  // k + 1's scores to sn.  ka / va: LDS addresses of stage k + 1's K and of stage k's V but
+  // for the constants OK / OV.
+  auto step = [&](int k, sf_f32x16& sc, sf_f32x16& sn, const sf_u32x4 (&pp)[2],
+                  sf_u32x4 (&pc)[2], const sf_lds_off (&ka)[8], auto OK, const sf_lds_off (&va)[4],
+                  auto OV) {
+    sf_u32x4 kf[8];
+    read_k<decltype(OK)::value>(ka, kf);
+    __builtin_amdgcn_sched_barrier(0);
+    if (resc) {   // what the step before decided: acc to the reference of its P
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) acc[dt] = acc[dt] * alpha;
+    }
+    const int key0 = keys.key0(c0 + k);
+    const bool masked = key0 + kStage > end_min || (key0 < lo_max && key0 + kStage > c.sinks);
+    if (masked) mask_scores(sc, key0, hf, end, lo, c.sinks);
+    // O^T += V^T P^T of stage k - 1: dim tiles d0 .. d1 of the keys 16kk
+    auto pv = [&](int kk, int d0, int d1) {
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+        if (dt >= d0 && dt < d1)
+          acc[dt] = mfma32(v_operand(vf, kk, dt), sf_as_bf16x8(pp[kk]), acc[dt]);
+    };
+    pv(0, 0, 2);
+    float mx = sc[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
+    mx *= scale_log2;
+    m_hi = fmaxf(m_hi, mx);
+    resc = __ballot(mx > m_ref + kLazy) != 0;   // wave-uniform
+    if (resc) {
+      m_hi = fmaxf(m_hi, __shfl_xor(m_hi, 32, 64));
+      alpha = __builtin_amdgcn_exp2f(m_ref - (m_hi == -INFINITY ? 0.f : m_hi));
+      m_ref = m_hi;
+      l_run *= alpha;
+    }
+    const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+    float p[16];
+    pv(0, 2, 4);
+    pv(1, 0, 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], scale_log2, -mu));
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, 3, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    sf_lds_reads_done(kf);
+    read_v<decltype(OV)::value>(va, vf);
+    __builtin_amdgcn_sched_barrier(0);
+    qk(kf, sn);
+#pragma unroll
+    for (int i = 8; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], scale_log2, -mu));
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) s0 += p[i], s1 += p[i + 1];
+    l_run += s0 + s1;
+    pack_p(p, pc);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, 6, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    sf_lds_reads_done(vf);
+    if (masked) bad = bad || any_not_finite(vf);
+  };
+
+  // Two stages a turn: slots 2i, 2i + 1 of the ring.  At the start of step k the stages to
+  // k + 1 have landed and every wave is through with stage k - 1's slot, which takes
+  // stage k + kAhead.
+#pragma unroll 1
+  for (int k = 0; k < nst; k += 2) {
+    const sf_lds_off b0 = sf_lds_addr(ring) + (k % kRing) * kSlot;
+    sf_lds_off ka[8], va[4];
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) ka[ks] = b0 + koff[ks];
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) va[dt] = b0 + voff[dt];
+    sf_wait_vm_barrier<(kAhead - 2) * kCopies>();
+    issue(k + kAhead);
+    step(k, sa, sb, pb, pa, ka, Int<kSlot>{}, va, Int<0>{});
+    if (k + 1 == nst) {   // (workgroup-uniform) the last: its P.V follows from the b side
+      pb[0] = pa[0];
+      pb[1] = pa[1];
+      break;
+    }
+    const sf_lds_off b1 = sf_lds_addr(ring) + ((k + 2) % kRing) * kSlot;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) ka[ks] = b1 + koff[ks];
+    sf_wait_vm_barrier<(kAhead - 2) * kCopies>();
+    issue(k + 1 + kAhead);
+    step(k + 1, sb, sa, pa, pb, ka, Int<0>{}, va, Int<kSlot>{});
+  }
+  sf_wait_vm_barrier<0>();   // drain the copies past the range's end
+  if (bad) {   // wave-uniform
+    slow_queries(q, c, s, it.h, it.r, q0, 32, keys, c0, nst, Out{o, lse, ws_o, ws_ml, scale_log2});
+    return;
+  }
+  if (resc) {
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) acc[dt] = acc[dt] * alpha;
+  }
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+      acc[dt] = mfma32(v_operand(vf, kk, dt), sf_as_bf16x8(pb[kk]), acc[dt]);
+
+  const float l = l_run + __shfl_xor(l_run, 32, 64);
+  if (q0 + (lane & 31) >= nq) return;
+  if (c.nr == 1) {
+    write_direct(acc, m_ref, l, hf, o + rh * kHD, lse ? lse + rh : nullptr);
+  } else {
+    const size_t slot = (size_t)it.r * c.rows * c.H + rh;
+    write_partial(acc, m_ref, l, hf, ws_o + slot * kHD, ws_ml + slot * 2);
+  }
+}
+
+// ---- up to 32 queries of a kv head (a token, or a few) ---------------------------------------
+// Bound by reading the cache once: each of the four waves takes every fourth stage of the
+// range with all the queries, through an LDS ring of its own (two stages, no workgroup
+// barrier), and the waves' states are joined at the end.
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void
+sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
+                     uint16_t* __restrict__ o, float* __restrict__ lse, float* __restrict__ ws_o,
+                     float* __restrict__ ws_ml) {
+  __shared__ __attribute__((aligned(16))) uint8_t ring[4 * 2 * kSlot];
+  __shared__ int s_pg[2 * (kMaxKeys / kStage)];
+  const Item it = find_item(c);
+  const Seq& s = c.s[it.si];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, hf = lane >> 5;
+  const int G = c.H / c.Hkv, nq = s.rows * G, P = s.length;
+  const Keys keys = query_tile_keys(0, 32, G, s.rows, P, c.block, c.window, c.sinks);
+  const int c0 = it.r * c.spr;
+  if (c0 >= keys.nst) return;
+  const int nst = min(c.spr, keys.nst - c0);
+  const int lastg = last_group(P);
+  if (s.table)
+    for (int i = tid; i < 2 * nst; i += kThreads)
+      s_pg[i] = page_of(s, c.page_shift, min(keys.key0(c0 + (i >> 1)) + 16 * (i & 1), lastg));
+  const int qi = min(lane & 31, nq - 1);
+  const int m = qi / G;
+  const int end = row_end(m, s.rows, P, c.block), lo = row_lo(m, s.rows, P, c.window);
+  const int end_min = row_end(0, s.rows, P, c.block);
+  const int lo_max = row_lo(s.rows - 1, s.rows, P, c.window);
+  const size_t rh = (size_t)(s.row0 + m) * c.H + it.h * G + (qi - m * G);
+  sf_u32x4 qf[8];
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks)
+    qf[ks] = *reinterpret_cast<const sf_u32x4*>(q + rh * kHD + 16 * ks + 8 * hf);
+  sf_wait_vm_loads();
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) sf_pin(qf[ks]);
+  __syncthreads();   // s_pg
+
+  uint8_t* mine = ring + wv * 2 * kSlot;
+  int uk[4], uv[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    uk[i] = copy_unit(lane, 4 * i, false), uv[i] = copy_unit(lane, 4 * i, true);
+  const uint16_t* kb = s.k + (long long)it.h * s.head_stride;
+  const uint16_t* vb = s.v + (long long)it.h * s.head_stride;
+  const sf_lds_off pg_addr = sf_lds_addr(s_pg);
+  auto issue = [&](int k, int slot) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int g0 = min(keys.key0(c0 + k) + 16 * g, lastg);
+      const int page = s.table ? __builtin_amdgcn_readfirstlane(
+                                     (int)sf_lds_read4_now(pg_addr + 4 * (2 * k + g)))
+                               : 0;
+      copy_rows<4>(kb, s, c.page_shift, page, g0, 0, uk, mine + slot * kSlot + 16 * g * kRowBytes);
+      copy_rows<4>(vb, s, c.page_shift, page, g0, 0, uv,
+                   mine + slot * kSlot + kHalf + 16 * g * kRowBytes);
+    }
+  };
+  if (wv < nst) {
+    issue(wv, 0);
+    issue(min(wv + 4, nst - 1), 1);
+  }
+  sf_lds_off ka[8], va[4];
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) ka[ks] = sf_lds_addr(mine) + k_off(lane, ks);
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) va[dt] = sf_lds_addr(mine) + v_off(lane, dt);
+
+  float m_ref = -INFINITY, l_run = 0.f;   // the query's reference: its running maximum
+  bool bad = false;
+  sf_f32x16 acc[4];
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
+
+  int slot = 0;
+#pragma unroll 1
+  for (int k = wv; k < nst; k += 4) {
+    wait_vm_wave<16>();   // this stage has landed; the next one (16 copies) may be on its way
+    sf_u32x4 kf[8];
+    sf_u32x2 vf[16];
+    sf_lds_off kc[8], vc[4];
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) kc[ks] = ka[ks] + slot * kSlot;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) vc[dt] = va[dt] + slot * kSlot;
+    read_k<0>(kc, kf);
+    read_v<0>(vc, vf);
+    sf_lds_reads_done_but<15>(kf);
+    sf_f32x16 sc;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks)
+      sc = mfma32(sf_as_bf16x8(kf[ks]), sf_as_bf16x8(qf[ks]), sc);
+    const int key0 = keys.key0(c0 + k);
+    const bool masked = key0 + kStage > end_min || (key0 < lo_max && key0 + kStage > c.sinks);
+    if (masked) mask_scores(sc, key0, hf, end, lo, c.sinks);
+    float mx = sc[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * scale_log2;
+    const float nm = fmaxf(m_ref, mx);
+    const float mu = nm == -INFINITY ? 0.f : nm;
+    const float alpha = __builtin_amdgcn_exp2f(m_ref - mu);
+    m_ref = nm;
+    float p[16], s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], scale_log2, -mu));
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) s0 += p[i], s1 += p[i + 1];
+    l_run = l_run * alpha + (s0 + s1);
+    sf_u32x4 pb[2];
+    pack_p(p, pb);
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) acc[dt] = acc[dt] * alpha;
+    sf_lds_reads_done(vf);
+    if (masked) bad = bad || any_not_finite(vf);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+        acc[dt] = mfma32(v_operand(vf, kk, dt), sf_as_bf16x8(pb[kk]), acc[dt]);
+    wait_vm_wave<16>();   // (no LDS read of the slot is left)
+    issue(min(k + 8, nst - 1), slot);
+    slot ^= 1;
+  }
+  l_run += __shfl_xor(l_run, 32, 64);
+  sf_wait_vm_barrier<0>();   // the ring is free: every copy landed, every wave done
+
+  // a hidden value that was not finite: the item again, a key at a time
+  if (lane == 0) s_pg[wv] = bad;
+  __syncthreads();
+  if (s_pg[0] | s_pg[1] | s_pg[2] | s_pg[3]) {   // workgroup-uniform
+    slow_queries(q, c, s, it.h, it.r, 8 * wv, 8, keys, c0, nst,
+                 Out{o, lse, ws_o, ws_ml, scale_log2});
+    return;
+  }
+
+  // join the four waves' states: waves 1..3 leave theirs in LDS
+  float* xo = reinterpret_cast<float*>(ring);           // [wave - 1][dt][4][lane] x 4
+  float* xml = xo + 3 * 4 * 4 * 64 * 4;                 // [wave - 1][query] x 2
+  if (wv > 0) {
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        *reinterpret_cast<sf_f32x4*>(xo + ((((wv - 1) * 4 + dt) * 4 + b) * 64 + lane) * 4) =
+            sf_f32x4{acc[dt][4 * b], acc[dt][4 * b + 1], acc[dt][4 * b + 2],
+                     acc[dt][4 * b + 3]};
+    if (hf == 0) {
+      xml[((wv - 1) * 32 + lane) * 2] = m_ref;
+      xml[((wv - 1) * 32 + lane) * 2 + 1] = l_run;
+    }
+  }
+  __syncthreads();
+  if (wv > 0) return;
+  float mm = m_ref;
+  float mw[3], lw[3];
+#pragma unroll
+  for (int w = 0; w < 3; ++w) {
+    mw[w] = xml[(w * 32 + (lane & 31)) * 2];
+    lw[w] = xml[(w * 32 + (lane & 31)) * 2 + 1];
+    mm = fmaxf(mm, mw[w]);
+  }
+  const float mu = mm == -INFINITY ? 0.f : mm;
+  const float w0 = __builtin_amdgcn_exp2f(m_ref - mu);
+  float l = l_run * w0;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) acc[dt] = acc[dt] * w0;
+#pragma unroll
+  for (int w = 0; w < 3; ++w) {
+    const float f = __builtin_amdgcn_exp2f(mw[w] - mu);
+    l += lw[w] * f;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const sf_f32x4 x = *reinterpret_cast<const sf_f32x4*>(
+            xo + (((w * 4 + dt) * 4 + b) * 64 + lane) * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[dt][4 * b + i] = fmaf(x[i], f, acc[dt][4 * b + i]);
+      }
+  }
+  if ((lane & 31) >= nq) return;
+  if (c.nr == 1) {
+    write_direct(acc, mm, l, hf, o + rh * kHD, lse ? lse + rh : nullptr);
+  } else {
+    const size_t slot_at = (size_t)it.r * c.rows * c.H + rh;
+    write_partial(acc, mm, l, hf, ws_o + slot_at * kHD, ws_ml + slot_at * 2);
+  }
+}
+
+// ---- join the ranges: one wave per (row, q-head), two dims a lane -----------------------------
+__global__ __launch_bounds__(kThreads) void sf_window_merge_kernel(Call c, int bq,
+                                                                   uint16_t* __restrict__ o,
+                                                                   float* __restrict__ lse,
+                                                                   const float* __restrict__ ws_o,
+                                                                   const float* __restrict__ ws_ml) {
   const int lane = threadIdx.x & 63;
   const int e = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (e >= c.rows * c.H) return;
   const int row = e / c.H, hq = e - row * c.H;
-  const int h = hq / (c.H / c.Hkv);
   int si = 0;
   while (row >= c.s[si].row0 + c.s[si].rows) ++si;
   const Seq& s = c.s[si];
-  const int m = row - s.row0;
-  const int end = row_end(c, s, m), lo = row_lo(c, s, m);
-  const uint16_t* qr = q + (size_t)row * c.H * kHD + hq * kHD;
-  float mx = -INFINITY, l = 0.f, a0 = 0.f, a1 = 0.f;
-  for (int t0 = 0; t0 < end; t0 += 64) {
-    if (t0 >= c.sinks && t0 + 64 <= lo) continue;
-    const int t = t0 + lane;
-    const bool see = t < end && (t < c.sinks || t >= lo);
-    float x = -INFINITY;
-    if (see) {
-      const uint16_t* kr = s.k + key_off(s, c.page_size, h, t);
-      x = 0.f;
-      for (int d = 0; d < kHD; d += 8) {
-        float a[8], b[8];
-        sf_unpack8(*reinterpret_cast<const sf_u32x4*>(kr + d), a);
-        sf_unpack8(*reinterpret_cast<const sf_u32x4*>(qr + d), b);
-        for (int i = 0; i < 8; ++i) x = fmaf(a[i], b[i], x);
+  if (s.tiles == 0) return;   // of the other launch
+  const int G = c.H / c.Hkv;
+  const int qi = (row - s.row0) * G + hq % G;
+  const Keys keys =
+      query_tile_keys(qi / bq, bq, G, s.rows, s.length, c.block, c.window, c.sinks);
+  const int nm = (keys.nst + c.spr - 1) / c.spr;   // <= nr <= 64
+  const size_t step = (size_t)c.rows * c.H;
+  const sf_f32x2 ml = sf_handoff_load(
+      reinterpret_cast<const sf_f32x2*>(ws_ml + (e + min(lane, nm - 1) * step) * 2));
+  const float mr = lane < nm ? ml.x : -INFINITY;
+  const float mm = sf_wave_max(mr);
+  const float mu = mm == -INFINITY ? 0.f : mm;
+  const float w = lane < nm ? __builtin_amdgcn_exp2f(mr - mu) : 0.f;
+  // (a range in which the row sees nothing: m -inf, l 0, acc 0)
+  const float l = sf_wave_sum(lane < nm ? ml.y * w : 0.f);
+  const float inv = 1.0f / l;
+  float ax = 0.f, ay = 0.f;
+  for (int r0 = 0; r0 < nm; r0 += 4) {
+    sf_f32x2 a[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      a[u] = sf_handoff_load(reinterpret_cast<const sf_f32x2*>(
+          ws_o + (e + min(r0 + u, nm - 1) * step) * kHD + 2 * lane));
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float wr = r0 + u < nm ? __shfl(w, min(r0 + u, 63), 64) : 0.f;
+      if (r0 + u < nm) {
+        ax = fmaf(wr, a[u].x, ax);
+        ay = fmaf(wr, a[u].y, ay);
       }
-      x *= scaling;
-    }
-    const float nm = fmaxf(mx, sf_wave_max(x));
-    const float ref = nm == -INFINITY ? 0.f : nm;
-    const float alpha = expf(mx - ref);
-    const float p = see ? expf(x - ref) : 0.f;
-    l = l * alpha + sf_wave_sum(p);
-    a0 *= alpha;
-    a1 *= alpha;
-    mx = nm;
-    unsigned long long bits = __ballot(see);
-    while (bits) {
-      const int j = __builtin_ctzll(bits);
-      bits &= bits - 1;
-      const float pj = __shfl(p, j, 64);
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(
-          s.v + key_off(s, c.page_size, h, t0 + j) + 2 * lane);
-      a0 = fmaf(pj, __uint_as_float(w << 16), a0);
-      a1 = fmaf(pj, __uint_as_float(w & 0xffff0000u), a1);
     }
   }
-  *reinterpret_cast<uint32_t*>(o + (size_t)row * c.H * kHD + hq * kHD + 2 * lane) =
-      sf_pack2(a0 / l, a1 / l);
-  if (lse && lane == 0) lse[(size_t)row * c.H + hq] = mx + logf(l);
+  *reinterpret_cast<uint32_t*>(o + (size_t)e * kHD + 2 * lane) = sf_pack2(ax * inv, ay * inv);
+  if (lse && lane == 0) lse[e] = mm * kLn2 + logf(l);
+}
+
+// ---- key mass --------------------------------------------------------------------------------
+struct MassSeq {
+  const float* in;
+  float* out;
+  long long in_stride, out_stride;
+};
+struct MassCall : Call {
+  MassSeq mass[kMaxSeqs];
+};
+SF_DEV long long key_off(const Seq& s, int page_shift, int h, int t) {
+  return (long long)h * s.head_stride +
+         (s.table ? page_of(s, page_shift, t) * s.page_stride +
+                        (long long)(t & ((1 << page_shift) - 1)) * kHD
+                  : (long long)t * kHD);
 }
 
 // One thread per (sequence, kv head, key).
 __global__ __launch_bounds__(256) void sf_window_mass_kernel(const uint16_t* __restrict__ q,
                                                              const float* __restrict__ lse,
-                                                             Call c, float scaling, float decay) {
+                                                             MassCall c, float scaling, float decay) {
   int tile = blockIdx.x, si = 0;
   for (; si < c.n_seqs; ++si) {
     const int nt = (c.s[si].length + 255) / 256;
@@ -118,15 +798,16 @@ __global__ __launch_bounds__(256) void sf_window_mass_kernel(const uint16_t* __r
   }
   if (si == c.n_seqs) return;
   const Seq& s = c.s[si];
+  const MassSeq& ms = c.mass[si];
   const int h = blockIdx.y, G = c.H / c.Hkv;
   const int t = tile * 256 + threadIdx.x;
   if (t >= s.length) return;
   sf_u32x4 kv[16];
-  const uint16_t* kr = s.k + key_off(s, c.page_size, h, t);
+  const uint16_t* kr = s.k + key_off(s, c.page_shift, h, t);
   for (int i = 0; i < 16; ++i) kv[i] = *reinterpret_cast<const sf_u32x4*>(kr + 8 * i);
   float sum = 0.f;
   for (int m = 0; m < s.rows; ++m) {
-    if (t >= row_end(c, s, m) || (t >= c.sinks && t < row_lo(c, s, m))) continue;
+    if (t >= row_end(m, s.rows, s.length, c.block) || (t >= c.sinks && t < row_lo(m, s.rows, s.length, c.window))) continue;
     for (int g = 0; g < G; ++g) {
       const size_t r = (size_t)(s.row0 + m) * c.H + h * G + g;
       float x = 0.f;
@@ -139,8 +820,8 @@ __global__ __launch_bounds__(256) void sf_window_mass_kernel(const uint16_t* __r
       sum += expf(x * scaling - lse[r]);
     }
   }
-  const float had = s.mass_in ? decay * s.mass_in[h * s.mass_in_stride + t] : 0.f;
-  s.mass_out[h * s.mass_out_stride + t] = had + sum;
+  const float had = ms.in ? decay * ms.in[h * ms.in_stride + t] : 0.f;
+  ms.out[h * ms.out_stride + t] = had + sum;
 }
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -153,7 +834,7 @@ int make_call(const sf_kv_seq* seqs, int n_seqs, int page_size, int block, int w
   if (block < 1 || window < 0 || sinks < 0) return SF_ERR_SHAPE;
   c = Call{};
   c.n_seqs = n_seqs;
-  c.page_size = page_size;
+  c.page_shift = page_size > 0 ? __builtin_ctz(page_size) : 0;
   c.block = block;
   c.window = window;
   c.sinks = sinks;
@@ -181,18 +862,62 @@ int make_call(const sf_kv_seq* seqs, int n_seqs, int page_size, int block, int w
         if (x.mass_in == x.mass_out && x.mass_in_stride != x.mass_out_stride) return SF_ERR_ARG;
       }
     }
-    c.s[i] = Seq{x.k, x.v, x.page_table, x.mass_in, x.mass_out, x.page_stride, x.head_stride,
-                 x.mass_in_stride, x.mass_out_stride, x.length, x.rows, c.rows, x.pages};
+    c.s[i] = Seq{x.k, x.v, x.page_table, x.page_stride, x.head_stride, x.length, x.rows, c.rows,
+                 x.pages, 0, 0};
     c.rows += x.rows;
   }
   return SF_OK;
+}
+
+// Cuts the tiles of the sequences with few_max < queries <= most into ranges for `slots`
+// workgroups at once, in stages: an item costs its stages and a fixed part (set-up, and
+// with several ranges its partial sums and their join).  The longest item, or the work
+// spread evenly and half an item of imbalance.
+struct Cost {
+  int one, many;   // stages' worth of an item's fixed part, in one range / several
+};
+int plan_ranges(Call& c, int bq, int least, int most, int slots, Cost fix) {
+  const int G = c.H / c.Hkv;
+  long long work = 0;
+  int longest = 0;
+  c.tiles = 0;
+  for (int i = 0; i < c.n_seqs; ++i) {
+    Seq& s = c.s[i];
+    const int nq = s.rows * G;
+    s.tile0 = c.tiles;
+    s.tiles = nq >= least && nq <= most ? tiles_of(s.rows, G, bq) : 0;
+    c.tiles += s.tiles;
+    for (int t = 0; t < s.tiles; ++t) {
+      const int n =
+          query_tile_keys(t, bq, G, s.rows, s.length, c.block, c.window, c.sinks).nst;
+      work += n;
+      longest = n > longest ? n : longest;
+    }
+  }
+  if (c.tiles == 0) return 0;
+  double best = 0;
+  const int cap = ranges_cap(c.rows);
+  for (int nr = 1; nr <= cap && nr <= longest; ++nr) {
+    const int spr = (longest + nr - 1) / nr;
+    const double items = c.Hkv * (nr == 1 ? (double)c.tiles : (double)work / spr + 0.5 * c.tiles);
+    const double one = spr + (nr == 1 ? fix.one : fix.many);
+    const double all = (c.Hkv * (double)work + items * (one - spr)) / slots;
+    const double cost = items <= slots ? one : all + 0.5 * one;
+    if (nr == 1 || cost < best) {
+      best = cost;
+      c.nr = (longest + spr - 1) / spr;
+      c.spr = spr;
+    }
+  }
+  return c.tiles * c.nr * c.Hkv;
 }
 
 }  // namespace
 
 extern "C" size_t sf_attn_window_workspace_bytes(int rows, int H) {
   if (rows < 0 || H < 1) return 0;
-  return 16;
+  if (rows == 0) return 16;
+  return (size_t)ranges_cap(rows) * rows * H * (kHD + 2) * sizeof(float);
 }
 
 extern "C" int sf_attn_window(const uint16_t* q, const sf_kv_seq* seqs, int n_seqs, int page_size,
@@ -206,8 +931,37 @@ extern "C" int sf_attn_window(const uint16_t* q, const sf_kv_seq* seqs, int n_se
   if (!q || !o || !workspace || !aligned(q) || !aligned(o) || !aligned(workspace))
     return SF_ERR_ARG;
   if (workspace_bytes < sf_attn_window_workspace_bytes(c.rows, H)) return SF_ERR_WORKSPACE;
-  hipLaunchKernelGGL(sf_window_attn_kernel, dim3((c.rows * H + 3) / 4), dim3(256), 0,
-                     reinterpret_cast<hipStream_t>(stream), q, c, scaling, o, lse);
+  hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+  const float scale_log2 = scaling * kLog2e;
+  float* ws_o = reinterpret_cast<float*>(workspace);
+  float* ws_ml = ws_o + (size_t)ranges_cap(c.rows) * c.rows * H * kHD;
+  const int G = H / Hkv;
+  // sequences of up to 32 queries a kv head, then the others
+  for (int few = 1; few >= 0; --few) {
+    int bq = 32, items;
+    if (few) {
+      items = plan_ranges(c, bq, 1, 32, kCUs, Cost{16, 24});
+    } else {
+      long long tiles = 0;
+      for (int i = 0; i < n_seqs; ++i)
+        if (c.s[i].rows * G > 32) tiles += tiles_of(c.s[i].rows, G, 256);
+      bq = tiles * Hkv >= kCUs ? 256 : 128;
+      items = plan_ranges(c, bq, 33, 1 << 30, bq == 256 ? kCUs : 2 * kCUs, Cost{4, 12});
+    }
+    if (items == 0) continue;
+    if (few)
+      hipLaunchKernelGGL(sf_window_few_kernel, dim3(items), dim3(kThreads), 0, hs, q, c,
+                         scale_log2, o, lse, ws_o, ws_ml);
+    else if (bq == 256)
+      hipLaunchKernelGGL((sf_window_tile_kernel<8>), dim3(items), dim3(512), 0, hs, q, c,
+                         scale_log2, o, lse, ws_o, ws_ml);
+    else
+      hipLaunchKernelGGL((sf_window_tile_kernel<4>), dim3(items), dim3(256), 0, hs, q, c,
+                         scale_log2, o, lse, ws_o, ws_ml);
+    if (c.nr > 1)
+      hipLaunchKernelGGL(sf_window_merge_kernel, dim3((c.rows * H + 3) / 4), dim3(kThreads), 0, hs,
+                         c, bq, o, lse, ws_o, ws_ml);
+  }
   return sf_launch_status();
 }
 
@@ -220,7 +974,7 @@ extern "C" int sf_attn_key_mass(const uint16_t* q, const float* lse, const sf_kv
                                 int n_seqs, int page_size, int block, int window, int sinks, int H,
                                 int Hkv, int hd, float scaling, float decay, void* workspace,
                                 size_t workspace_bytes, void* stream) {
-  Call c;
+  MassCall c;
   const int st = make_call(seqs, n_seqs, page_size, block, window, sinks, H, Hkv, hd, true, c);
   if (st != SF_OK) return st;
   if (!(decay >= 0.f && decay <= 1.f)) return SF_ERR_ARG;
@@ -228,6 +982,8 @@ extern "C" int sf_attn_key_mass(const uint16_t* q, const float* lse, const sf_kv
   int keys = 0, tiles = 0;
   for (int i = 0; i < n_seqs; ++i) {
     keys += c.s[i].length;
+    c.mass[i] = MassSeq{seqs[i].mass_in, seqs[i].mass_out, seqs[i].mass_in_stride,
+                        seqs[i].mass_out_stride};
     tiles += (c.s[i].length + 255) / 256;
   }
   if (keys == 0) return SF_OK;

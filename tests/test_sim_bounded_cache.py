@@ -299,7 +299,7 @@ def test_evict_refusals(over, code):
 
 def test_wrapper_refusals(sim):
     q, ks, vs, caches = make_seqs([(3, 20)], 4, 2, 1, "cpu")
-    o, ws = torch.empty(3, 512, dtype=BF), torch.empty(1 << 16, dtype=torch.uint8)
+    o, ws = torch.empty(3, 512, dtype=BF), torch.empty(1 << 23, dtype=torch.uint8)
     batch = PagedBatch(caches, [3])
     with pytest.raises(TypeError):
         sim.attn_window(q.float(), batch, 0, 4, 0.1, o, ws)

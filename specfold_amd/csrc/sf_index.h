@@ -560,6 +560,36 @@ SF_IDX Keys query_tile_keys(int t, int bq, int G, int n, int P, int block, int w
   return tile_keys(t * bq / G, q1 / G, n, P, block, window, sinks);
 }
 
+// Rows [m0, m1) see a key of [k0, k1] (m1 <= m0: none do).
+struct Rows {
+  int m0, m1;
+};
+SF_IDX Rows seen_rows(int k0, int k1, int n, int P, int block, int window, int sinks) {
+  const int first = P - n;   // the rows' own keys from here
+  Rows r{k0 < first ? 0 : (k0 - first) / block * block, n};
+  if (window > 0 && k0 >= sinks) {
+    const long long m1 = (long long)k1 + window - first;   // row_lo(m) <= k1
+    r.m1 = m1 < 0 ? 0 : m1 < n ? (int)m1 : n;
+  }
+  return r;
+}
+// Key mass: keys in tiles of 256; 32-query stages of the queries that see a tile.
+constexpr int kMassKeys = 256;
+constexpr int kMassRanges = 16;   // ranges of queries at most (bounds the workspace)
+SF_IDX int mass_stages(const Rows& r, int G) { return r.m1 > r.m0 ? ((r.m1 - r.m0) * G + 31) / 32 : 0; }
+
+// x / d by a multiplication, for 0 <= x < 2^20 and 1 <= d <= 2^15 with x * d < 2^32
+// (ceil(2^32 / d) is off by less than 1 / 2^32 of x * d from x / d's next step).
+struct Div {
+  unsigned d, mul;
+  SF_IDX int of(int x) const {
+    return d == 1 ? x : (int)(((unsigned long long)(unsigned)x * mul) >> 32);
+  }
+};
+inline Div make_div(int d) {
+  return Div{(unsigned)d, d == 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d)};
+}
+
 // Ranges a query's keys are cut into at most, by the rows of the call (bounds the
 // workspace of partial sums: 4096 row partials, or 4 of every row).
 SF_IDX int ranges_cap(int rows) { return rows >= 1024 ? 4 : (rows <= 64 ? 64 : 4096 / rows); }

@@ -771,57 +771,250 @@ __global__ __launch_bounds__(kThreads) void sf_window_merge_kernel(Call c, int b
 }
 
 // ---- key mass --------------------------------------------------------------------------------
+// A workgroup sums the weights of 256 keys (wave w: 64 of them, K operands in registers)
+// over a range of the queries that see them, 32 at a time through an LDS ring: S^T = K Q^T
+// as above, so a lane adds up the weights one of every 32 queries gives to 32 keys, and the
+// lanes are joined every 32 stages, in a fixed order: the error of one fp32 chain over all
+// of them would grow with the queries.  The step of stage i runs the weights of stage i
+// beside S^T of stage i + 1.  Bound by the
+// exponentials (a quarter-rate operation per score) for many rows, by reading K for few.
 struct MassSeq {
   const float* in;
   float* out;
   long long in_stride, out_stride;
+  int key0;   // its first key's place in a row of partial sums
 };
 struct MassCall : Call {
   MassSeq mass[kMaxSeqs];
+  Div div_g, div_block;
+  int keys;   // of all sequences
 };
-SF_DEV long long key_off(const Seq& s, int page_shift, int h, int t) {
-  return (long long)h * s.head_stride +
-         (s.table ? page_of(s, page_shift, t) * s.page_stride +
-                        (long long)(t & ((1 << page_shift) - 1)) * kHD
-                  : (long long)t * kHD);
+// 4 bytes per lane of a direct copy, and an LDS read of 4 bytes without a wait.
+#if defined(__HIPCC__)
+SF_DEV void lds_dma4(const void* src, void* lds_base) {
+  __builtin_amdgcn_global_load_lds(const_cast<void*>(src), (sf_lds_void*)lds_base, 4, 0, 0);
+}
+SF_DEV uint32_t lds_read4(sf_lds_off addr) {
+  uint32_t v;
+  asm volatile("ds_read_b32 %0, %1" : "=v"(v) : "v"(addr));
+  return v;
+}
+#else
+inline void lds_dma4(const void* src, void* lds_base) {
+  __builtin_memcpy(static_cast<char*>(lds_base) + 4 * sim_lane(), src, 4);
+}
+inline uint32_t lds_read4(sf_lds_off addr) { return sf_lds_read4_now(addr); }
+#endif
+
+constexpr int kQSlot = 32 * kRowBytes;   // 32 queries: 8 KB
+constexpr int kMassRing = 4;             // slot 0 of its own, the others over the K rows
+constexpr int kFlush = 32;               // stages summed lane by lane
+
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ lse, MassCall c,
+                      float scale_log2, float decay, float* __restrict__ ws) {
+  // K rows of the four waves (16 KB each), slot 0, the stages' lse (256 bytes a slot)
+  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * 2 * kHalf + kQSlot + kMassRing * 256];
+  const Item it = find_item(c);
+  const Seq& s = c.s[it.si];
+  const MassSeq& ms = c.mass[it.si];
+  const int tile = s.tiles - 1 - it.tile;   // the first keys (the most rows) first
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, hf = lane >> 5;
+  const int G = c.H / c.Hkv, P = s.length, n = s.rows;
+  const int k0 = tile * kMassKeys;
+  const Rows rows = seen_rows(k0, min(k0 + kMassKeys, P) - 1, n, P, c.block, c.window, c.sinks);
+  const int all = mass_stages(rows, G);
+  const int i0 = it.r * c.spr;
+  if (i0 >= all && it.r > 0) return;
+  const int nst = max(0, min(c.spr, all - i0));
+  const int qb = rows.m0 * G + 32 * i0, q_end = rows.m1 * G;
+  const int kw0 = k0 + 64 * wv;   // the wave's first key
+  // row_end by a multiplication
+  auto end_of = [&](int m) { return P - n + min(n, (c.div_block.of(m) + 1) * (int)c.div_block.d); };
+  auto q_at = [&](int qi) {
+    const int m = c.div_g.of(qi);
+    return (size_t)(s.row0 + m) * c.H + it.h * G + (qi - m * G);
+  };
+
+  uint8_t* const kmine = lds + wv * 2 * kHalf;
+  uint8_t* const lse_at = lds + 4 * 2 * kHalf + kQSlot;
+  auto slot = [&](int i) {
+    return i % kMassRing == 0 ? lds + 4 * 2 * kHalf : lds + (i % kMassRing - 1) * kQSlot;
+  };
+  // stage i's queries (wave w: 8 rows) and their lse: past the range its last stage again,
+  // past the queries the last query
+  auto issue = [&](int i) {
+    const int q0 = qb + 32 * min(i, nst - 1);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r0 = 8 * wv + 4 * u;
+      sf_lds_dma16(q + q_at(min(q0 + r0 + (lane >> 4), q_end - 1)) * kHD +
+                       copy_unit(lane, r0, false),
+                   slot(i) + r0 * kRowBytes);
+    }
+    // (every wave its own copy of the lse would cost LDS: all write the same values)
+    lds_dma4(lse + q_at(min(q0 + (lane & 31), q_end - 1)), lse_at + 256 * (i % kMassRing));
+  };
+
+  float acc[2][16], total = 0.f;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
+  // acc joined over the lanes and added to the total of this lane's key: lane x of a half
+  // ends with value x of the 32 (key tile x / 16)
+  auto flush = [&]() {
+    float v[32];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[16 * t + j] = acc[t][j], acc[t][j] = 0.f;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+      const bool up = lane & o;
+#pragma unroll
+      for (int x = 0; x < o; ++x) {
+        const float give = up ? v[x] : v[x + o], keep = up ? v[x + o] : v[x];
+        v[x] = keep + __shfl_xor(give, o, 64);
+      }
+    }
+    total += v[0];
+  };
+
+  if (nst > 0) {   // workgroup-uniform
+    // ---- the wave's 64 keys, stage 0, then the K operands to registers --------------------
+    {
+      const int lastg = last_group(P);
+      const uint16_t* kb = s.k + (long long)it.h * s.head_stride;
+      int unit[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) unit[i] = copy_unit(lane, 4 * i, false);
+      int page[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        page[g] = s.table ? page_of(s, c.page_shift, min(kw0 + 16 * g, lastg)) : 0;
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        copy_rows<4>(kb, s, c.page_shift, __builtin_amdgcn_readfirstlane(page[g]),
+                     min(kw0 + 16 * g, lastg), 0, unit, kmine + 16 * g * kRowBytes);
+    }
+    issue(0);
+    sf_wait_vm_barrier<0>();
+    uint32_t koff[8];
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) koff[ks] = k_off(lane, ks);
+    sf_u32x4 kf[2][8];
+    {
+      sf_lds_off ka[8];
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) ka[ks] = sf_lds_addr(kmine) + koff[ks];
+      read_k<0>(ka, kf[0]);
+      read_k<kHalf>(ka, kf[1]);
+      sf_lds_reads_done(kf[0]);
+      sf_lds_reads_done(kf[1]);
+    }
+    sf_lds_barrier();   // the K rows make room for slots 1 ..
+#pragma unroll
+    for (int i = 1; i < kMassRing - 1; ++i) issue(i);
+
+    const sf_lds_off lse_addr = sf_lds_addr(lse_at) + 4 * lane;
+    // S^T of a stage (both key tiles) and its queries' -lse in base 2
+    auto scores = [&](int i, sf_f32x16 (&out)[2], float& nl) {
+      sf_lds_off ka[8];
+      const sf_lds_off b = sf_lds_addr(slot(i));
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) ka[ks] = b + koff[ks];
+      sf_u32x4 qf[8];
+      read_k<0>(ka, qf);
+      uint32_t w = lds_read4(lse_addr + 256 * (i % kMassRing));
+      sf_lds_reads_done(qf);
+      sf_pin(w);
+      nl = -kLog2e * __uint_as_float(w);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) out[t][j] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          out[t] = mfma32(sf_as_bf16x8(kf[t][ks]), sf_as_bf16x8(qf[ks]), out[t]);
+    };
+    auto step = [&](int i, sf_f32x16 (&sc)[2], const float& nl, sf_f32x16 (&sn)[2], float& nn) {
+      // stage i + 1 has landed, and every wave is through with stage i - 1's slot
+      sf_wait_vm_barrier<(kMassRing - 3) * 3>();
+      issue(i + kMassRing - 1);
+      scores(i + 1, sn, nn);
+      const int q0 = qb + 32 * i;
+      const int m_first = c.div_g.of(q0), m_last = c.div_g.of(min(q0 + 31, q_end - 1));
+      const bool skip = end_of(m_last) <= kw0 ||
+                        (kw0 >= c.sinks && row_lo(m_first, n, P, c.window) > kw0 + 63);
+      const bool full = q0 + 31 < q_end && end_of(m_first) >= min(kw0 + 64, P) &&
+                        (kw0 + 63 < c.sinks || row_lo(m_last, n, P, c.window) <= kw0);
+      if (full) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            acc[t][j] += __builtin_amdgcn_exp2f(fmaf(sc[t][j], scale_log2, nl));
+      } else if (!skip) {
+        const int qi = q0 + (lane & 31);
+        const int m = c.div_g.of(min(qi, q_end - 1));
+        const int end = qi < q_end ? end_of(m) : 0;
+        const int lo = qi < q_end ? row_lo(m, n, P, c.window) : 0;
+        const int sinks = qi < q_end ? c.sinks : 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int key = kw0 + 32 * t + 8 * (j >> 2) + 4 * hf + (j & 3);
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[t][j], scale_log2, nl));
+            acc[t][j] += key < end && (key >= lo || key < sinks) ? p : 0.f;
+          }
+      }
+    };
+    sf_f32x16 sa[2], sb[2];
+    float na, nb;
+    scores(0, sa, na);
+#pragma unroll 1
+    for (int i = 0; i < nst; i += 2) {
+      step(i, sa, na, sb, nb);
+      if (i + 1 < nst) step(i + 1, sb, nb, sa, na);
+      if ((i & (kFlush - 1)) == kFlush - 2) flush();
+    }
+    sf_wait_vm_barrier<0>();   // drain the copies past the range's end
+  }
+
+  flush();
+  const int x = lane & 31;
+  const int key = kw0 + 32 * (x >> 4) + 8 * ((x & 15) >> 2) + 4 * hf + (x & 3);
+  if (key >= P) return;
+  if (c.nr == 1) {
+    const float had = ms.in ? decay * ms.in[it.h * ms.in_stride + key] : 0.f;
+    ms.out[it.h * ms.out_stride + key] = had + total;
+  } else {
+    sf_handoff_store(ws + ((size_t)it.r * c.Hkv + it.h) * c.keys + ms.key0 + key, total);
+  }
 }
 
-// One thread per (sequence, kv head, key).
-__global__ __launch_bounds__(256) void sf_window_mass_kernel(const uint16_t* __restrict__ q,
-                                                             const float* __restrict__ lse,
-                                                             MassCall c, float scaling, float decay) {
-  int tile = blockIdx.x, si = 0;
-  for (; si < c.n_seqs; ++si) {
-    const int nt = (c.s[si].length + 255) / 256;
-    if (tile < nt) break;
-    tile -= nt;
-  }
-  if (si == c.n_seqs) return;
+// the ranges' sums in order, and what the key had
+__global__ __launch_bounds__(kMassKeys) void sf_window_mass_merge_kernel(
+    MassCall c, float decay, const float* __restrict__ ws) {
+  const int h = blockIdx.x % c.Hkv, tt = blockIdx.x / c.Hkv;
+  int si = 0;
+  while (tt >= c.s[si].tile0 + c.s[si].tiles) ++si;
   const Seq& s = c.s[si];
   const MassSeq& ms = c.mass[si];
-  const int h = blockIdx.y, G = c.H / c.Hkv;
-  const int t = tile * 256 + threadIdx.x;
-  if (t >= s.length) return;
-  sf_u32x4 kv[16];
-  const uint16_t* kr = s.k + key_off(s, c.page_shift, h, t);
-  for (int i = 0; i < 16; ++i) kv[i] = *reinterpret_cast<const sf_u32x4*>(kr + 8 * i);
+  const int k0 = (tt - s.tile0) * kMassKeys, key = k0 + threadIdx.x;
+  if (key >= s.length) return;
+  const Rows rows = seen_rows(k0, min(k0 + kMassKeys, s.length) - 1, s.rows, s.length, c.block,
+                              c.window, c.sinks);
+  const int nm = (mass_stages(rows, c.H / c.Hkv) + c.spr - 1) / c.spr;
   float sum = 0.f;
-  for (int m = 0; m < s.rows; ++m) {
-    if (t >= row_end(m, s.rows, s.length, c.block) || (t >= c.sinks && t < row_lo(m, s.rows, s.length, c.window))) continue;
-    for (int g = 0; g < G; ++g) {
-      const size_t r = (size_t)(s.row0 + m) * c.H + h * G + g;
-      float x = 0.f;
-      for (int i = 0; i < 16; ++i) {
-        float a[8], b[8];
-        sf_unpack8(kv[i], a);
-        sf_unpack8(*reinterpret_cast<const sf_u32x4*>(q + r * kHD + 8 * i), b);
-        for (int j = 0; j < 8; ++j) x = fmaf(a[j], b[j], x);
-      }
-      sum += expf(x * scaling - lse[r]);
-    }
-  }
-  const float had = ms.in ? decay * ms.in[h * ms.in_stride + t] : 0.f;
-  ms.out[h * ms.out_stride + t] = had + sum;
+  for (int r = 0; r < nm; ++r)
+    sum += sf_handoff_load(ws + ((size_t)r * c.Hkv + h) * c.keys + ms.key0 + key);
+  const float had = ms.in ? decay * ms.in[h * ms.in_stride + key] : 0.f;
+  ms.out[h * ms.out_stride + key] = had + sum;
 }
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -869,13 +1062,29 @@ int make_call(const sf_kv_seq* seqs, int n_seqs, int page_size, int block, int w
   return SF_OK;
 }
 
-// Cuts the tiles of the sequences with few_max < queries <= most into ranges for `slots`
-// workgroups at once, in stages: an item costs its stages and a fixed part (set-up, and
-// with several ranges its partial sums and their join).  The longest item, or the work
-// spread evenly and half an item of imbalance.
+// Ranges of the tiles for `slots` workgroups at once, in stages: an item costs its stages
+// and a fixed part (set-up, and with several ranges its partial sums and their join).  The
+// longest item, or the work spread evenly and half an item of imbalance.
 struct Cost {
   int one, many;   // stages' worth of an item's fixed part, in one range / several
 };
+void plan_spread(Call& c, long long work, int longest, int cap, int slots, Cost fix) {
+  double best = 0;
+  for (int nr = 1; nr <= cap && nr <= longest; ++nr) {
+    const int spr = (longest + nr - 1) / nr;
+    const double items = c.Hkv * (nr == 1 ? (double)c.tiles : (double)work / spr + 0.5 * c.tiles);
+    const double one = spr + (nr == 1 ? fix.one : fix.many);
+    const double all = (c.Hkv * (double)work + items * (one - spr)) / slots;
+    const double cost = items <= slots ? one : all + 0.5 * one;
+    if (nr == 1 || cost < best) {
+      best = cost;
+      c.nr = (longest + spr - 1) / spr;
+      c.spr = spr;
+    }
+  }
+}
+
+// The tiles of the sequences with least to most queries a kv head, and their ranges.
 int plan_ranges(Call& c, int bq, int least, int most, int slots, Cost fix) {
   const int G = c.H / c.Hkv;
   long long work = 0;
@@ -895,20 +1104,7 @@ int plan_ranges(Call& c, int bq, int least, int most, int slots, Cost fix) {
     }
   }
   if (c.tiles == 0) return 0;
-  double best = 0;
-  const int cap = ranges_cap(c.rows);
-  for (int nr = 1; nr <= cap && nr <= longest; ++nr) {
-    const int spr = (longest + nr - 1) / nr;
-    const double items = c.Hkv * (nr == 1 ? (double)c.tiles : (double)work / spr + 0.5 * c.tiles);
-    const double one = spr + (nr == 1 ? fix.one : fix.many);
-    const double all = (c.Hkv * (double)work + items * (one - spr)) / slots;
-    const double cost = items <= slots ? one : all + 0.5 * one;
-    if (nr == 1 || cost < best) {
-      best = cost;
-      c.nr = (longest + spr - 1) / spr;
-      c.spr = spr;
-    }
-  }
+  plan_spread(c, work, longest, ranges_cap(c.rows), slots, fix);
   return c.tiles * c.nr * c.Hkv;
 }
 
@@ -967,7 +1163,7 @@ extern "C" int sf_attn_window(const uint16_t* q, const sf_kv_seq* seqs, int n_se
 
 extern "C" size_t sf_attn_key_mass_workspace_bytes(int keys, int Hkv) {
   if (keys < 0 || Hkv < 1) return 0;
-  return 16;
+  return keys == 0 ? 16 : (size_t)kMassRanges * Hkv * keys * sizeof(float);
 }
 
 extern "C" int sf_attn_key_mass(const uint16_t* q, const float* lse, const sf_kv_seq* seqs,
@@ -979,17 +1175,38 @@ extern "C" int sf_attn_key_mass(const uint16_t* q, const float* lse, const sf_kv
   if (st != SF_OK) return st;
   if (!(decay >= 0.f && decay <= 1.f)) return SF_ERR_ARG;
   if (c.rows > 0 && (!q || !lse || !aligned(q))) return SF_ERR_ARG;
-  int keys = 0, tiles = 0;
+  c.div_g = make_div(H / Hkv);
+  c.div_block = make_div(block < kMaxKeys ? block : kMaxKeys);
+  // tiles and their stages; ranges as plan_ranges: the longest item, or the work spread
+  long long work = 0;
+  int longest = 1;
+  c.keys = c.tiles = 0;
   for (int i = 0; i < n_seqs; ++i) {
-    keys += c.s[i].length;
+    Seq& s = c.s[i];
     c.mass[i] = MassSeq{seqs[i].mass_in, seqs[i].mass_out, seqs[i].mass_in_stride,
-                        seqs[i].mass_out_stride};
-    tiles += (c.s[i].length + 255) / 256;
+                        seqs[i].mass_out_stride, c.keys};
+    c.keys += s.length;
+    s.tile0 = c.tiles;
+    s.tiles = (s.length + kMassKeys - 1) / kMassKeys;
+    c.tiles += s.tiles;
+    for (int t = 0; t < s.tiles; ++t) {
+      const int k1 = (t + 1) * kMassKeys < s.length ? (t + 1) * kMassKeys : s.length;
+      const int n = mass_stages(
+          seen_rows(t * kMassKeys, k1 - 1, s.rows, s.length, block, window, sinks), H / Hkv);
+      work += n;
+      longest = n > longest ? n : longest;
+    }
   }
-  if (keys == 0) return SF_OK;
+  if (c.keys == 0) return SF_OK;
   if (!workspace || !aligned(workspace)) return SF_ERR_ARG;
-  if (workspace_bytes < sf_attn_key_mass_workspace_bytes(keys, Hkv)) return SF_ERR_WORKSPACE;
-  hipLaunchKernelGGL(sf_window_mass_kernel, dim3(tiles, Hkv), dim3(256), 0,
-                     reinterpret_cast<hipStream_t>(stream), q, lse, c, scaling, decay);
+  if (workspace_bytes < sf_attn_key_mass_workspace_bytes(c.keys, Hkv)) return SF_ERR_WORKSPACE;
+  plan_spread(c, work, longest, kMassRanges, 2 * kCUs, Cost{6, 10});
+  hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+  float* ws = reinterpret_cast<float*>(workspace);
+  hipLaunchKernelGGL(sf_window_mass_kernel, dim3(c.tiles * c.nr * Hkv), dim3(kThreads), 0, hs, q,
+                     lse, c, scaling * kLog2e, decay, ws);
+  if (c.nr > 1)
+    hipLaunchKernelGGL(sf_window_mass_merge_kernel, dim3(c.tiles * Hkv), dim3(kMassKeys), 0, hs, c,
+                       decay, ws);
   return sf_launch_status();
 }

@@ -77,9 +77,9 @@ struct Call {
   int tiles, nr, spr;      // tiles of all sequences, ranges of a tile, stages of a range
 };
 
+SF_DEV int page_in(const Seq& s, int id) { return id >= 0 && id < s.pages ? id : 0; }
 SF_DEV int page_of(const Seq& s, int page_shift, int key) {
-  const int id = s.table[key >> page_shift];
-  return id >= 0 && id < s.pages ? id : 0;
+  return page_in(s, s.table[key >> page_shift]);
 }
 
 // ---- LDS stages ------------------------------------------------------------------------
@@ -313,7 +313,6 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   constexpr int kAhead = kRing - 1;
   constexpr int kCopies = 16 / W;   // of a wave per stage: 4 rows each
   __shared__ __attribute__((aligned(16))) uint8_t ring[kRing * kSlot];
-  __shared__ int s_pg[2 * (kMaxKeys / kStage) + 64];
   const Item it = find_item(c);
   const Seq& s = c.s[it.si];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, hf = lane >> 5;
@@ -325,10 +324,13 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   const int nst = min(c.spr, keys.nst - c0);
   const int lastg = last_group(P);
 
-  // the page of every 16-key group of the range; the queries
-  if (s.table)
-    for (int i = tid; i < 2 * nst; i += 64 * W)
-      s_pg[i] = page_of(s, c.page_shift, min(keys.key0(c0 + (i >> 1)) + 16 * (i & 1), lastg));
+  // lane i: the page table's entry for 16-key group i & 1 of stage 32u + i / 2 of the range
+  auto load_pages = [&](int u) {
+    const int k = min(32 * u + (lane >> 1), nst - 1);
+    return s.table[min(keys.key0(c0 + k) + 16 * (lane & 1), lastg) >> c.page_shift];
+  };
+  int pg = 0, pg_next = 0;   // of the 32 stages being copied, and the 32 behind them
+  if (s.table) pg_next = load_pages(0);
   const int q0 = it.tile * kBQ + wv * 32;   // the wave's first query
   const int qi = min(q0 + (lane & 31), nq - 1);   // padding: the last query again
   const int m = qi / G;
@@ -344,7 +346,6 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   sf_wait_vm_loads();
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks) sf_pin(qf[ks]);
-  __syncthreads();   // s_pg
 
   // copies: 16-key group wv * 4 / W of K0, K1, V0, V1
   const int part = wv * 4 / W, grp = part & 1;
@@ -354,13 +355,17 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   int unit_off[kCopies];
 #pragma unroll
   for (int i = 0; i < kCopies; ++i) unit_off[i] = copy_unit(lane, row0 + 4 * i, is_v);
-  const sf_lds_off pg_addr = sf_lds_addr(s_pg) + 4 * lane;
-  int pg = 0;   // lane i: the page of group i of the 32 stages being copied
   auto issue = [&](int k) {
     const int kc = min(k, nst - 1);   // past the range: its last stage again
-    if (s.table && (k & 31) == 0) pg = (int)sf_lds_read4_now(pg_addr + 4 * 64 * (kc >> 5));
+    int page = 0;
+    if (s.table) {
+      if ((k & 31) == 0) {
+        pg = pg_next;
+        pg_next = load_pages((k >> 5) + 1);
+      }
+      page = page_in(s, lane_value(pg, 2 * (k & 31) + grp));
+    }
     const int g0 = min(keys.key0(c0 + kc) + 16 * grp, lastg);
-    const int page = s.table ? lane_value(pg, 2 * (kc & 31) + grp) : 0;
     copy_rows<kCopies>(base, s, c.page_shift, page, g0, row0, unit_off,
                        ring + (k % kRing) * kSlot + (is_v ? kHalf : 0) + 16 * grp * kRowBytes);
   };
@@ -530,14 +535,15 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
 
 // ---- up to 32 queries of a kv head (a token, or a few) ---------------------------------------
 // Bound by reading the cache once: each of the four waves takes every fourth stage of the
-// range with all the queries, through an LDS ring of its own (two stages, no workgroup
-// barrier), and the waves' states are joined at the end.
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void
+// range with all the queries, through an LDS slot of its own (no workgroup barrier): a
+// stage's operands go to registers as soon as it has landed, and the slot takes the next
+// one.  Two workgroups a CU: 128 KB on their way.  The waves' states are joined at the end.
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
 sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
                      uint16_t* __restrict__ o, float* __restrict__ lse, float* __restrict__ ws_o,
                      float* __restrict__ ws_ml) {
-  __shared__ __attribute__((aligned(16))) uint8_t ring[4 * 2 * kSlot];
-  __shared__ int s_pg[2 * (kMaxKeys / kStage)];
+  __shared__ __attribute__((aligned(16))) uint8_t ring[4 * kSlot];
+  __shared__ int s_bad[4];
   const Item it = find_item(c);
   const Seq& s = c.s[it.si];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, hf = lane >> 5;
@@ -547,9 +553,12 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   if (c0 >= keys.nst) return;
   const int nst = min(c.spr, keys.nst - c0);
   const int lastg = last_group(P);
-  if (s.table)
-    for (int i = tid; i < 2 * nst; i += kThreads)
-      s_pg[i] = page_of(s, c.page_shift, min(keys.key0(c0 + (i >> 1)) + 16 * (i & 1), lastg));
+  // lane i: the page table's entry for 16-key group i & 1 of this wave's stage 32u + i / 2
+  auto load_pages = [&](int u) {
+    const int k = min(wv + 4 * (32 * u + (lane >> 1)), nst - 1);
+    return s.table[min(keys.key0(c0 + k) + 16 * (lane & 1), lastg) >> c.page_shift];
+  };
+  int pg = s.table ? load_pages(0) : 0;
   const int qi = min(lane & 31, nq - 1);
   const int m = qi / G;
   const int end = row_end(m, s.rows, P, c.block), lo = row_lo(m, s.rows, P, c.window);
@@ -560,35 +569,26 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks)
     qf[ks] = *reinterpret_cast<const sf_u32x4*>(q + rh * kHD + 16 * ks + 8 * hf);
-  sf_wait_vm_loads();
-#pragma unroll
-  for (int ks = 0; ks < 8; ++ks) sf_pin(qf[ks]);
-  __syncthreads();   // s_pg
 
-  uint8_t* mine = ring + wv * 2 * kSlot;
+  uint8_t* mine = ring + wv * kSlot;
   int uk[4], uv[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     uk[i] = copy_unit(lane, 4 * i, false), uv[i] = copy_unit(lane, 4 * i, true);
   const uint16_t* kb = s.k + (long long)it.h * s.head_stride;
   const uint16_t* vb = s.v + (long long)it.h * s.head_stride;
-  const sf_lds_off pg_addr = sf_lds_addr(s_pg);
-  auto issue = [&](int k, int slot) {
+  auto issue = [&](int j) {   // this wave's stage j
+    const int key0 = keys.key0(c0 + wv + 4 * j);
+    if (s.table && j > 0 && (j & 31) == 0) pg = load_pages(j >> 5);
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      const int g0 = min(keys.key0(c0 + k) + 16 * g, lastg);
-      const int page = s.table ? __builtin_amdgcn_readfirstlane(
-                                     (int)sf_lds_read4_now(pg_addr + 4 * (2 * k + g)))
-                               : 0;
-      copy_rows<4>(kb, s, c.page_shift, page, g0, 0, uk, mine + slot * kSlot + 16 * g * kRowBytes);
-      copy_rows<4>(vb, s, c.page_shift, page, g0, 0, uv,
-                   mine + slot * kSlot + kHalf + 16 * g * kRowBytes);
+      const int g0 = min(key0 + 16 * g, lastg);
+      const int page = s.table ? page_in(s, lane_value(pg, 2 * (j & 31) + g)) : 0;
+      copy_rows<4>(kb, s, c.page_shift, page, g0, 0, uk, mine + 16 * g * kRowBytes);
+      copy_rows<4>(vb, s, c.page_shift, page, g0, 0, uv, mine + kHalf + 16 * g * kRowBytes);
     }
   };
-  if (wv < nst) {
-    issue(wv, 0);
-    issue(min(wv + 4, nst - 1), 1);
-  }
+  if (wv < nst) issue(0);
   sf_lds_off ka[8], va[4];
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks) ka[ks] = sf_lds_addr(mine) + k_off(lane, ks);
@@ -603,27 +603,24 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
 
-  int slot = 0;
 #pragma unroll 1
-  for (int k = wv; k < nst; k += 4) {
-    wait_vm_wave<16>();   // this stage has landed; the next one (16 copies) may be on its way
+  for (int j = 0; wv + 4 * j < nst; ++j) {
+    wait_vm_wave<0>();   // the stage (and the queries) have landed
     sf_u32x4 kf[8];
     sf_u32x2 vf[16];
-    sf_lds_off kc[8], vc[4];
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks) kc[ks] = ka[ks] + slot * kSlot;
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt) vc[dt] = va[dt] + slot * kSlot;
-    read_k<0>(kc, kf);
-    read_v<0>(vc, vf);
-    sf_lds_reads_done_but<15>(kf);
+    read_k<0>(ka, kf);
+    read_v<0>(va, vf);
+    sf_lds_reads_done(kf);
+    sf_lds_reads_done(vf);
+    wait_vm_wave<63>();   // (every lane has read)
+    if (wv + 4 * (j + 1) < nst) issue(j + 1);
     sf_f32x16 sc;
 #pragma unroll
     for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks)
       sc = mfma32(sf_as_bf16x8(kf[ks]), sf_as_bf16x8(qf[ks]), sc);
-    const int key0 = keys.key0(c0 + k);
+    const int key0 = keys.key0(c0 + wv + 4 * j);
     const bool masked = key0 + kStage > end_min || (key0 < lo_max && key0 + kStage > c.sinks);
     if (masked) mask_scores(sc, key0, hf, end, lo, c.sinks);
     float mx = sc[0];
@@ -644,24 +641,20 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
     pack_p(p, pb);
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) acc[dt] = acc[dt] * alpha;
-    sf_lds_reads_done(vf);
     if (masked) bad = bad || any_not_finite(vf);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt)
         acc[dt] = mfma32(v_operand(vf, kk, dt), sf_as_bf16x8(pb[kk]), acc[dt]);
-    wait_vm_wave<16>();   // (no LDS read of the slot is left)
-    issue(min(k + 8, nst - 1), slot);
-    slot ^= 1;
   }
   l_run += __shfl_xor(l_run, 32, 64);
   sf_wait_vm_barrier<0>();   // the ring is free: every copy landed, every wave done
 
   // a hidden value that was not finite: the item again, a key at a time
-  if (lane == 0) s_pg[wv] = bad;
+  if (lane == 0) s_bad[wv] = bad;
   __syncthreads();
-  if (s_pg[0] | s_pg[1] | s_pg[2] | s_pg[3]) {   // workgroup-uniform
+  if (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) {   // workgroup-uniform
     slow_queries(q, c, s, it.h, it.r, 8 * wv, 8, keys, c0, nst,
                  Out{o, lse, ws_o, ws_ml, scale_log2});
     return;
@@ -721,7 +714,8 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   }
 }
 
-// ---- join the ranges: one wave per (row, q-head), two dims a lane -----------------------------
+// ---- join the ranges: one wave per (row, q-head), two dims a lane, NB ranges on their way ------
+template <int NB>
 __global__ __launch_bounds__(kThreads) void sf_window_merge_kernel(Call c, int bq,
                                                                    uint16_t* __restrict__ o,
                                                                    float* __restrict__ lse,
@@ -741,6 +735,14 @@ __global__ __launch_bounds__(kThreads) void sf_window_merge_kernel(Call c, int b
       query_tile_keys(qi / bq, bq, G, s.rows, s.length, c.block, c.window, c.sinks);
   const int nm = (keys.nst + c.spr - 1) / c.spr;   // <= nr <= 64
   const size_t step = (size_t)c.rows * c.H;
+  sf_f32x2 a[NB];
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < NB; ++u)
+      a[u] = sf_handoff_load(reinterpret_cast<const sf_f32x2*>(
+          ws_o + (e + min(r0 + u, nm - 1) * step) * kHD + 2 * lane));
+  };
+  load(0);
   const sf_f32x2 ml = sf_handoff_load(
       reinterpret_cast<const sf_f32x2*>(ws_ml + (e + min(lane, nm - 1) * step) * 2));
   const float mr = lane < nm ? ml.x : -INFINITY;
@@ -751,16 +753,12 @@ __global__ __launch_bounds__(kThreads) void sf_window_merge_kernel(Call c, int b
   const float l = sf_wave_sum(lane < nm ? ml.y * w : 0.f);
   const float inv = 1.0f / l;
   float ax = 0.f, ay = 0.f;
-  for (int r0 = 0; r0 < nm; r0 += 4) {
-    sf_f32x2 a[4];
+  for (int r0 = 0; r0 < nm; r0 += NB) {
+    if (r0 > 0) load(r0);
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      a[u] = sf_handoff_load(reinterpret_cast<const sf_f32x2*>(
-          ws_o + (e + min(r0 + u, nm - 1) * step) * kHD + 2 * lane));
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float wr = r0 + u < nm ? __shfl(w, min(r0 + u, 63), 64) : 0.f;
-      if (r0 + u < nm) {
+    for (int u = 0; u < NB; ++u) {
+      if (r0 + u < nm) {   // wave-uniform
+        const float wr = __shfl(w, r0 + u, 64);
         ax = fmaf(wr, a[u].x, ax);
         ay = fmaf(wr, a[u].y, ay);
       }
@@ -1136,13 +1134,14 @@ extern "C" int sf_attn_window(const uint16_t* q, const sf_kv_seq* seqs, int n_se
   for (int few = 1; few >= 0; --few) {
     int bq = 32, items;
     if (few) {
-      items = plan_ranges(c, bq, 1, 32, kCUs, Cost{16, 24});
+      items = plan_ranges(c, bq, 1, 32, 2 * kCUs, Cost{12, 20});
     } else {
       long long tiles = 0;
       for (int i = 0; i < n_seqs; ++i)
         if (c.s[i].rows * G > 32) tiles += tiles_of(c.s[i].rows, G, 256);
       bq = tiles * Hkv >= kCUs ? 256 : 128;
-      items = plan_ranges(c, bq, 33, 1 << 30, bq == 256 ? kCUs : 2 * kCUs, Cost{4, 12});
+      items = plan_ranges(c, bq, 33, 1 << 30, bq == 256 ? kCUs : 2 * kCUs,
+                          bq == 256 ? Cost{4, 34} : Cost{6, 24});
     }
     if (items == 0) continue;
     if (few)
@@ -1154,9 +1153,12 @@ extern "C" int sf_attn_window(const uint16_t* q, const sf_kv_seq* seqs, int n_se
     else
       hipLaunchKernelGGL((sf_window_tile_kernel<4>), dim3(items), dim3(256), 0, hs, q, c,
                          scale_log2, o, lse, ws_o, ws_ml);
-    if (c.nr > 1)
-      hipLaunchKernelGGL(sf_window_merge_kernel, dim3((c.rows * H + 3) / 4), dim3(kThreads), 0, hs,
-                         c, bq, o, lse, ws_o, ws_ml);
+    if (c.nr > 4)
+      hipLaunchKernelGGL((sf_window_merge_kernel<16>), dim3((c.rows * H + 3) / 4), dim3(kThreads),
+                         0, hs, c, bq, o, lse, ws_o, ws_ml);
+    else if (c.nr > 1)
+      hipLaunchKernelGGL((sf_window_merge_kernel<4>), dim3((c.rows * H + 3) / 4), dim3(kThreads),
+                         0, hs, c, bq, o, lse, ws_o, ws_ml);
   }
   return sf_launch_status();
 }

@@ -103,32 +103,51 @@ SF_DEV uint32_t v_off(int lane, int dt) {
   return (uint32_t)(kHalf + r * kRowBytes + (u ^ (2 * (r & 7))) * 16 + (lane & 1) * 8);
 }
 
+// Where the copies of a wave read: the pages of one kv head's K or V.  (Wave-uniform, in
+// registers: fields read through the argument would be loaded again in every stage.)
+struct Source {
+  const uint16_t* base;
+  const int32_t* table;
+  long long page_stride;
+  int pages, length, page_mask;
+};
+SF_DEV Source source_of(const uint16_t* kv, const Seq& s, int h, int page_shift) {
+  return Source{kv + (long long)h * s.head_stride, s.table, s.page_stride, s.pages, s.length,
+                (1 << page_shift) - 1};
+}
 // Copies rows row0 .. + 4 N of the 16-key group that starts at key g0 to a stage, `dst`
-// the group's first row there: keys behind the last repeat it.  page: the group's page.
+// the group's first row there: keys behind the last repeat it.  id: the page table's entry
+// of the group; off: copy i's element offset of this lane, row (row0 + 4i + lane / 16) *
+// kHD + copy_unit.
 template <int N>
-SF_DEV void copy_rows(const uint16_t* base, const Seq& s, int page_shift, int page, int g0,
-                      int row0, const int (&unit_off)[N], uint8_t* dst) {
-  const int lane = threadIdx.x & 63;
-  const uint16_t* src = base + (s.table ? (long long)page * s.page_stride +
-                                              (long long)(g0 & ((1 << page_shift) - 1)) * kHD
-                                        : (long long)g0 * kHD);
+SF_DEV void copy_rows(const Source& s, int id, int g0, int row0, const uint32_t (&off)[N],
+                      uint8_t* dst) {
+  const int page = id >= 0 && id < s.pages ? id : 0;
+  const uint16_t* src = s.base + (s.table ? (long long)page * s.page_stride +
+                                                (long long)(g0 & s.page_mask) * kHD
+                                          : (long long)g0 * kHD);
   const int last = s.length - 1 - g0;
   if (last >= 15) {   // wave-uniform
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      sf_lds_dma16(src + (row0 + 4 * i + (lane >> 4)) * kHD + unit_off[i],
-                   dst + (row0 + 4 * i) * kRowBytes);
+    for (int i = 0; i < N; ++i) sf_lds_dma16(src + off[i], dst + (row0 + 4 * i) * kRowBytes);
   } else {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      sf_lds_dma16(src + min(row0 + 4 * i + (lane >> 4), last) * kHD + unit_off[i],
-                   dst + (row0 + 4 * i) * kRowBytes);
+    for (int i = 0; i < N; ++i) {
+      const int over = max(0, row0 + 4 * i + (lane >> 4) - last);
+      sf_lds_dma16(src + ((int)off[i] - over * kHD), dst + (row0 + 4 * i) * kRowBytes);
+    }
   }
 }
 // the logical unit (in elements) that this lane's copy of rows r0 .. + 4 brings
 SF_DEV int copy_unit(int lane, int r0, bool is_v) {
   const int r = r0 + (lane >> 4), p = lane & 15;
   return (is_v ? p ^ (2 * (r & 7)) : p ^ (r & 15)) * 8;
+}
+
+// copy_rows' offset of this lane for rows r0 .. + 4
+SF_DEV uint32_t copy_off(int lane, int r0, bool is_v) {
+  return (uint32_t)((r0 + (lane >> 4)) * kHD + copy_unit(lane, r0, is_v));
 }
 
 SF_DEV int last_group(int P) { return (P - 1) & ~15; }
@@ -141,13 +160,16 @@ SF_DEV void pack_p(const float (&p)[16], sf_u32x4 (&pb)[2]) {
     for (int w = 0; w < 4; ++w) pb[kk][w] = sf_pack2(p[8 * kk + 2 * w], p[8 * kk + 2 * w + 1]);
 }
 
+SF_DEV bool seen_key(int key, int end, int lo, int sinks) {   // (lo <= end)
+  return ((unsigned)(key - lo) < (unsigned)(end - lo)) | ((key < sinks) & (key < end));
+}
 // The mask of a stage's scores for one query: keys at or behind `end`, and keys of
 // [sinks, lo).
 SF_DEV void mask_scores(sf_f32x16& s, int key0, int hf, int end, int lo, int sinks) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int key = key0 + 8 * (i >> 2) + 4 * hf + (i & 3);
-    if (key >= end || (key < lo && key >= sinks)) s[i] = -INFINITY;
+    s[i] = seen_key(key, end, lo, sinks) ? s[i] : -INFINITY;
   }
 }
 
@@ -315,7 +337,8 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   __shared__ __attribute__((aligned(16))) uint8_t ring[kRing * kSlot];
   const Item it = find_item(c);
   const Seq& s = c.s[it.si];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, hf = lane >> 5;
+  const int lane = threadIdx.x & 63, hf = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // wave-uniform
   const int G = c.H / c.Hkv, nq = s.rows * G, P = s.length;
   constexpr int kBQ = 32 * W;
   const Keys keys = query_tile_keys(it.tile, kBQ, G, s.rows, P, c.block, c.window, c.sinks);
@@ -324,13 +347,14 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   const int nst = min(c.spr, keys.nst - c0);
   const int lastg = last_group(P);
 
+  const int32_t* const table = s.table;
   // lane i: the page table's entry for 16-key group i & 1 of stage 32u + i / 2 of the range
   auto load_pages = [&](int u) {
     const int k = min(32 * u + (lane >> 1), nst - 1);
-    return s.table[min(keys.key0(c0 + k) + 16 * (lane & 1), lastg) >> c.page_shift];
+    return table[min(keys.key0(c0 + k) + 16 * (lane & 1), lastg) >> c.page_shift];
   };
   int pg = 0, pg_next = 0;   // of the 32 stages being copied, and the 32 behind them
-  if (s.table) pg_next = load_pages(0);
+  if (table) pg_next = load_pages(0);
   const int q0 = it.tile * kBQ + wv * 32;   // the wave's first query
   const int qi = min(q0 + (lane & 31), nq - 1);   // padding: the last query again
   const int m = qi / G;
@@ -351,23 +375,20 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   const int part = wv * 4 / W, grp = part & 1;
   const bool is_v = part >= 2;
   const int row0 = W == 8 ? 8 * (wv & 1) : 0;   // of the group
-  const uint16_t* base = (is_v ? s.v : s.k) + (long long)it.h * s.head_stride;
-  int unit_off[kCopies];
+  const Source src = source_of(is_v ? s.v : s.k, s, it.h, c.page_shift);
+  uint32_t off[kCopies];
 #pragma unroll
-  for (int i = 0; i < kCopies; ++i) unit_off[i] = copy_unit(lane, row0 + 4 * i, is_v);
+  for (int i = 0; i < kCopies; ++i) off[i] = copy_off(lane, row0 + 4 * i, is_v);
+  uint8_t* const dst = ring + (is_v ? kHalf : 0) + 16 * grp * kRowBytes;
   auto issue = [&](int k) {
     const int kc = min(k, nst - 1);   // past the range: its last stage again
-    int page = 0;
-    if (s.table) {
-      if ((k & 31) == 0) {
-        pg = pg_next;
-        pg_next = load_pages((k >> 5) + 1);
-      }
-      page = page_in(s, lane_value(pg, 2 * (k & 31) + grp));
+    if (src.table && (k & 31) == 0) {
+      pg = pg_next;
+      pg_next = load_pages((k >> 5) + 1);
     }
-    const int g0 = min(keys.key0(c0 + kc) + 16 * grp, lastg);
-    copy_rows<kCopies>(base, s, c.page_shift, page, g0, row0, unit_off,
-                       ring + (k % kRing) * kSlot + (is_v ? kHalf : 0) + 16 * grp * kRowBytes);
+    copy_rows<kCopies>(src, lane_value(pg, 2 * (k & 31) + grp),
+                       min(keys.key0(c0 + kc) + 16 * grp, lastg), row0, off,
+                       dst + (k % kRing) * kSlot);
   };
 #pragma unroll 1
   for (int k = 0; k < kAhead; ++k) issue(k);
@@ -455,6 +476,9 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
     pv(1, 0, 4);
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], scale_log2, -mu));
+    // (pinned: the compiler would take them to their use, behind all the MFMAs)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sf_pin(p[i]);
 #pragma unroll
     for (int i = 0; i < 6; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -472,6 +496,9 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
     for (int i = 0; i < 16; i += 2) s0 += p[i], s1 += p[i + 1];
     l_run += s0 + s1;
     pack_p(p, pc);
+    sf_pin(l_run);
+    sf_pin(pc[0]);
+    sf_pin(pc[1]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -546,19 +573,21 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   __shared__ int s_bad[4];
   const Item it = find_item(c);
   const Seq& s = c.s[it.si];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, hf = lane >> 5;
+  const int lane = threadIdx.x & 63, hf = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // wave-uniform
   const int G = c.H / c.Hkv, nq = s.rows * G, P = s.length;
   const Keys keys = query_tile_keys(0, 32, G, s.rows, P, c.block, c.window, c.sinks);
   const int c0 = it.r * c.spr;
   if (c0 >= keys.nst) return;
   const int nst = min(c.spr, keys.nst - c0);
   const int lastg = last_group(P);
+  const int32_t* const table = s.table;
   // lane i: the page table's entry for 16-key group i & 1 of this wave's stage 32u + i / 2
   auto load_pages = [&](int u) {
     const int k = min(wv + 4 * (32 * u + (lane >> 1)), nst - 1);
-    return s.table[min(keys.key0(c0 + k) + 16 * (lane & 1), lastg) >> c.page_shift];
+    return table[min(keys.key0(c0 + k) + 16 * (lane & 1), lastg) >> c.page_shift];
   };
-  int pg = s.table ? load_pages(0) : 0;
+  int pg = table ? load_pages(0) : 0;
   const int qi = min(lane & 31, nq - 1);
   const int m = qi / G;
   const int end = row_end(m, s.rows, P, c.block), lo = row_lo(m, s.rows, P, c.window);
@@ -571,21 +600,21 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
     qf[ks] = *reinterpret_cast<const sf_u32x4*>(q + rh * kHD + 16 * ks + 8 * hf);
 
   uint8_t* mine = ring + wv * kSlot;
-  int uk[4], uv[4];
+  uint32_t ok[4], ov[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    uk[i] = copy_unit(lane, 4 * i, false), uv[i] = copy_unit(lane, 4 * i, true);
-  const uint16_t* kb = s.k + (long long)it.h * s.head_stride;
-  const uint16_t* vb = s.v + (long long)it.h * s.head_stride;
+    ok[i] = copy_off(lane, 4 * i, false), ov[i] = copy_off(lane, 4 * i, true);
+  const Source sk = source_of(s.k, s, it.h, c.page_shift);
+  const Source sv = source_of(s.v, s, it.h, c.page_shift);
   auto issue = [&](int j) {   // this wave's stage j
     const int key0 = keys.key0(c0 + wv + 4 * j);
-    if (s.table && j > 0 && (j & 31) == 0) pg = load_pages(j >> 5);
+    if (table && j > 0 && (j & 31) == 0) pg = load_pages(j >> 5);
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const int g0 = min(key0 + 16 * g, lastg);
-      const int page = s.table ? page_in(s, lane_value(pg, 2 * (j & 31) + g)) : 0;
-      copy_rows<4>(kb, s, c.page_shift, page, g0, 0, uk, mine + 16 * g * kRowBytes);
-      copy_rows<4>(vb, s, c.page_shift, page, g0, 0, uv, mine + kHalf + 16 * g * kRowBytes);
+      const int id = lane_value(pg, 2 * (j & 31) + g);
+      copy_rows<4>(sk, id, g0, 0, ok, mine + 16 * g * kRowBytes);
+      copy_rows<4>(sv, id, g0, 0, ov, mine + kHalf + 16 * g * kRowBytes);
     }
   };
   if (wv < nst) issue(0);
@@ -817,7 +846,8 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
   const Seq& s = c.s[it.si];
   const MassSeq& ms = c.mass[it.si];
   const int tile = s.tiles - 1 - it.tile;   // the first keys (the most rows) first
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, hf = lane >> 5;
+  const int lane = threadIdx.x & 63, hf = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // wave-uniform
   const int G = c.H / c.Hkv, P = s.length, n = s.rows;
   const int k0 = tile * kMassKeys;
   const Rows rows = seen_rows(k0, min(k0 + kMassKeys, P) - 1, n, P, c.block, c.window, c.sinks);
@@ -883,18 +913,18 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
     // ---- the wave's 64 keys, stage 0, then the K operands to registers --------------------
     {
       const int lastg = last_group(P);
-      const uint16_t* kb = s.k + (long long)it.h * s.head_stride;
-      int unit[4];
+      const Source src = source_of(s.k, s, it.h, c.page_shift);
+      uint32_t off[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) unit[i] = copy_unit(lane, 4 * i, false);
-      int page[4];
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        page[g] = s.table ? page_of(s, c.page_shift, min(kw0 + 16 * g, lastg)) : 0;
+      for (int i = 0; i < 4; ++i) off[i] = copy_off(lane, 4 * i, false);
+      int id[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        copy_rows<4>(kb, s, c.page_shift, __builtin_amdgcn_readfirstlane(page[g]),
-                     min(kw0 + 16 * g, lastg), 0, unit, kmine + 16 * g * kRowBytes);
+        id[g] = s.table ? s.table[min(kw0 + 16 * g, lastg) >> c.page_shift] : 0;
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        copy_rows<4>(src, __builtin_amdgcn_readfirstlane(id[g]), min(kw0 + 16 * g, lastg), 0, off,
+                     kmine + 16 * g * kRowBytes);
     }
     issue(0);
     sf_wait_vm_barrier<0>();
@@ -967,7 +997,7 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
           for (int j = 0; j < 16; ++j) {
             const int key = kw0 + 32 * t + 8 * (j >> 2) + 4 * hf + (j & 3);
             const float p = __builtin_amdgcn_exp2f(fmaf(sc[t][j], scale_log2, nl));
-            acc[t][j] += key < end && (key >= lo || key < sinks) ? p : 0.f;
+            acc[t][j] += seen_key(key, end, lo, sinks) ? p : 0.f;
           }
       }
     };

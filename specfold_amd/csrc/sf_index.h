@@ -542,6 +542,12 @@ struct Keys {
   int sink_st, lo_st, nst;
   SF_IDX int stage(int i) const { return i < sink_st ? i : lo_st + i - sink_st; }
   SF_IDX int key0(int i) const { return stage(i) * kStage; }
+  // the first i whose stage starts at or behind `key`
+  SF_IDX int stage_of(int key) const {
+    const int st = key <= 0 ? 0 : (key + kStage - 1) / kStage;
+    if (st <= sink_st) return st;
+    return sink_st + sf_imax(0, st - lo_st);
+  }
 };
 SF_IDX Keys tile_keys(int m0, int m1, int n, int P, int block, int window, int sinks) {
   const int st_end = (row_end(m1, n, P, block) + kStage - 1) / kStage;

@@ -30,6 +30,7 @@ constexpr int kMaxKeys = 32768;
 constexpr int kMaxG = 16;
 constexpr int kThreads = 256;
 constexpr int kCUs = 256;
+constexpr int kTileQ = 128;   // queries of a tile
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLazy = 8.f;   // base-2 headroom of the softmax reference
@@ -103,41 +104,30 @@ SF_DEV uint32_t v_off(int lane, int dt) {
   return (uint32_t)(kHalf + r * kRowBytes + (u ^ (2 * (r & 7))) * 16 + (lane & 1) * 8);
 }
 
-// Where the copies of a wave read: the pages of one kv head's K or V.  (Wave-uniform, in
-// registers: fields read through the argument would be loaded again in every stage.)
-struct Source {
-  const uint16_t* base;
-  const int32_t* table;
-  long long page_stride;
-  int pages, length, page_mask;
-};
-SF_DEV Source source_of(const uint16_t* kv, const Seq& s, int h, int page_shift) {
-  return Source{kv + (long long)h * s.head_stride, s.table, s.page_stride, s.pages, s.length,
-                (1 << page_shift) - 1};
+// Element offset of the 16-key group that starts at key g0 from its kv head's first row; id:
+// the page table's entry of the group.
+SF_DEV long long group_off(const Seq& s, int page_shift, int id, int g0) {
+  if (!s.table) return (long long)g0 * kHD;
+  return page_in(s, id) * s.page_stride + (long long)(g0 & ((1 << page_shift) - 1)) * kHD;
 }
-// Copies rows row0 .. + 4 N of the 16-key group that starts at key g0 to a stage, `dst`
-// the group's first row there: keys behind the last repeat it.  id: the page table's entry
-// of the group; off: copy i's element offset of this lane, row (row0 + 4i + lane / 16) *
-// kHD + copy_unit.
-template <int N>
-SF_DEV void copy_rows(const Source& s, int id, int g0, int row0, const uint32_t (&off)[N],
-                      uint8_t* dst) {
-  const int page = id >= 0 && id < s.pages ? id : 0;
-  const uint16_t* src = s.base + (s.table ? (long long)page * s.page_stride +
-                                                (long long)(g0 & s.page_mask) * kHD
-                                          : (long long)g0 * kHD);
-  const int last = s.length - 1 - g0;
-  if (last >= 15) {   // wave-uniform
-#pragma unroll
-    for (int i = 0; i < N; ++i) sf_lds_dma16(src + off[i], dst + (row0 + 4 * i) * kRowBytes);
-  } else {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int over = max(0, row0 + 4 * i + (lane >> 4) - last);
-      sf_lds_dma16(src + ((int)off[i] - over * kHD), dst + (row0 + 4 * i) * kRowBytes);
-    }
+// The offsets of 64 groups, one a lane; lane i's as a wave-uniform value.
+struct Groups {
+  int lo, hi;
+  SF_DEV void set(long long off) {
+    lo = (int)(uint32_t)off;
+    hi = (int)(off >> 32);
   }
+  SF_DEV long long at(int i) const {
+    return (long long)((unsigned long long)(uint32_t)lane_value(hi, i) << 32 |
+                       (uint32_t)lane_value(lo, i));
+  }
+};
+// Copies 4 N rows of a group to a stage: off: copy i's element offset of this lane, its row
+// (4i + lane / 16 of them) * kHD + copy_unit.
+template <int N>
+SF_DEV void copy_rows(const uint16_t* src, const uint32_t (&off)[N], uint8_t* dst) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) sf_lds_dma16(src + off[i], dst + 4 * i * kRowBytes);
 }
 // the logical unit (in elements) that this lane's copy of rows r0 .. + 4 brings
 SF_DEV int copy_unit(int lane, int r0, bool is_v) {
@@ -145,9 +135,9 @@ SF_DEV int copy_unit(int lane, int r0, bool is_v) {
   return (is_v ? p ^ (2 * (r & 7)) : p ^ (r & 15)) * 8;
 }
 
-// copy_rows' offset of this lane for rows r0 .. + 4
-SF_DEV uint32_t copy_off(int lane, int r0, bool is_v) {
-  return (uint32_t)((r0 + (lane >> 4)) * kHD + copy_unit(lane, r0, is_v));
+// copy_rows' offset of this lane for rows r0 .. + 4, rows behind `last` repeating it
+SF_DEV uint32_t copy_off(int lane, int r0, bool is_v, int last) {
+  return (uint32_t)(min(r0 + (lane >> 4), last) * kHD + copy_unit(lane, r0, is_v));
 }
 
 SF_DEV int last_group(int P) { return (P - 1) & ~15; }
@@ -320,42 +310,41 @@ SF_DEV Item find_item(const Call& c) {
   return it;
 }
 
-// ---- tiles of 32 W queries -----------------------------------------------------------------
-// W waves, two on each SIMD (W = 8: one workgroup a CU, W = 4: two), wave w the queries
-// 32 w .. + 32 of the tile, all walking the same stages through an LDS ring that direct
-// copies fill kAhead stages ahead.  The step of stage k runs three independent things
-// side by side within the wave, the matrix core's and the vector ALU's: the softmax of
-// stage k, O^T += V^T P^T of stage k - 1 and S^T of stage k + 1.
-template <int W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+// ---- tiles of 128 queries ------------------------------------------------------------------
+// Four waves, wave w the queries 32 w .. + 32 of the tile, all walking the same stages
+// through an LDS ring that direct copies fill three stages ahead (wave w: the 16-key group
+// w & 1 of K or V).  The step of stage k runs three independent things side by side within
+// the wave, the matrix core's and the vector ALU's: the softmax of stage k, O^T += V^T P^T
+// of stage k - 1 and S^T of stage k + 1.  Two workgroups share a CU and drift apart, so
+// that one's matrix products meet the other's loads; one workgroup of eight waves and 256
+// queries, which copies half as much, measured 506 against 499 us on 8192 rows of 28 / 4
+// heads and 175 against 150 on four shorter runs of rows.
+constexpr int kRing = 4;
+constexpr int kAhead = kRing - 1;
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
 sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
                       uint16_t* __restrict__ o, float* __restrict__ lse, float* __restrict__ ws_o,
                       float* __restrict__ ws_ml) {
-  constexpr int kRing = W;
-  constexpr int kAhead = kRing - 1;
-  constexpr int kCopies = 16 / W;   // of a wave per stage: 4 rows each
   __shared__ __attribute__((aligned(16))) uint8_t ring[kRing * kSlot];
   const Item it = find_item(c);
   const Seq& s = c.s[it.si];
   const int lane = threadIdx.x & 63, hf = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // wave-uniform
   const int G = c.H / c.Hkv, nq = s.rows * G, P = s.length;
-  constexpr int kBQ = 32 * W;
-  const Keys keys = query_tile_keys(it.tile, kBQ, G, s.rows, P, c.block, c.window, c.sinks);
+  const Keys keys = query_tile_keys(it.tile, kTileQ, G, s.rows, P, c.block, c.window, c.sinks);
   const int c0 = it.r * c.spr;
   if (c0 >= keys.nst) return;
   const int nst = min(c.spr, keys.nst - c0);
   const int lastg = last_group(P);
 
-  const int32_t* const table = s.table;
-  // lane i: the page table's entry for 16-key group i & 1 of stage 32u + i / 2 of the range
-  auto load_pages = [&](int u) {
-    const int k = min(32 * u + (lane >> 1), nst - 1);
-    return table[min(keys.key0(c0 + k) + 16 * (lane & 1), lastg) >> c.page_shift];
+  // lane i: 16-key group i & 1 of stage 32u + i / 2 of the range (past it: its last stage)
+  auto lane_group = [&](int u) {
+    return min(keys.key0(c0 + min(32 * u + (lane >> 1), nst - 1)) + 16 * (lane & 1), lastg);
   };
-  int pg = 0, pg_next = 0;   // of the 32 stages being copied, and the 32 behind them
-  if (table) pg_next = load_pages(0);
-  const int q0 = it.tile * kBQ + wv * 32;   // the wave's first query
+  // ... and the page table's entry of it
+  auto load_pages = [&](int u) { return s.table ? s.table[lane_group(u) >> c.page_shift] : 0; };
+  int pg_next = load_pages(0);
+  const int q0 = it.tile * kTileQ + wv * 32;   // the wave's first query
   const int qi = min(q0 + (lane & 31), nq - 1);   // padding: the last query again
   const int m = qi / G;
   const int end = row_end(m, s.rows, P, c.block), lo = row_lo(m, s.rows, P, c.window);
@@ -371,24 +360,30 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks) sf_pin(qf[ks]);
 
-  // copies: 16-key group wv * 4 / W of K0, K1, V0, V1
-  const int part = wv * 4 / W, grp = part & 1;
-  const bool is_v = part >= 2;
-  const int row0 = W == 8 ? 8 * (wv & 1) : 0;   // of the group
-  const Source src = source_of(is_v ? s.v : s.k, s, it.h, c.page_shift);
-  uint32_t off[kCopies];
+  // copies: group wv & 1 of K (wv < 2) or V
+  const int grp = wv & 1;
+  const bool is_v = wv >= 2;
+  const uint16_t* const base = (is_v ? s.v : s.k) + (long long)it.h * s.head_stride;
+  // (off_last: of the last group of the cache, which may hold fewer than 16 keys)
+  uint32_t off[4], off_last[4];
 #pragma unroll
-  for (int i = 0; i < kCopies; ++i) off[i] = copy_off(lane, row0 + 4 * i, is_v);
+  for (int i = 0; i < 4; ++i) {
+    off[i] = copy_off(lane, 4 * i, is_v, 15);
+    off_last[i] = copy_off(lane, 4 * i, is_v, P - 1 - lastg);
+  }
   uint8_t* const dst = ring + (is_v ? kHalf : 0) + 16 * grp * kRowBytes;
-  auto issue = [&](int k) {
-    const int kc = min(k, nst - 1);   // past the range: its last stage again
-    if (src.table && (k & 31) == 0) {
-      pg = pg_next;
+  const int k_last = keys.stage_of(lastg - 16 * grp) - c0;   // from this stage on
+  Groups groups;   // of the 32 stages being copied
+  auto issue = [&](int k) {   // past the range: its last stage again
+    if ((k & 31) == 0) {
+      groups.set(group_off(s, c.page_shift, pg_next, lane_group(k >> 5)));
       pg_next = load_pages((k >> 5) + 1);
     }
-    copy_rows<kCopies>(src, lane_value(pg, 2 * (k & 31) + grp),
-                       min(keys.key0(c0 + kc) + 16 * grp, lastg), row0, off,
-                       dst + (k % kRing) * kSlot);
+    const bool last = k >= k_last;   // wave-uniform
+    uint32_t of[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) of[i] = last ? off_last[i] : off[i];
+    copy_rows<4>(base + groups.at(2 * (k & 31) + grp), of, dst + (k % kRing) * kSlot);
   };
 #pragma unroll 1
   for (int k = 0; k < kAhead; ++k) issue(k);
@@ -400,9 +395,10 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   for (int dt = 0; dt < 4; ++dt) voff[dt] = v_off(lane, dt);
 
   // online softmax per query: acc and l_run are kept against the reference m_ref (-inf:
-  // nothing yet), which moves up to the running maximum m_hi only when a score passes it
-  // by more than kLazy; m_hi and l_run are per lane (its own keys).
-  float m_ref = -INFINITY, m_hi = -INFINITY, l_run = 0.f, alpha = 1.f;
+  // nothing yet; mu: m_ref, or 0), which moves up to a stage's maximum only when that
+  // passes it by more than kLazy, so every exponential is at most 2^kLazy; l_run is per
+  // lane (its own keys).
+  float m_ref = -INFINITY, m_lim = -INFINITY, mu = 0.f, l_run = 0.f, alpha = 1.f;
   sf_f32x16 acc[4], sa, sb;
   sf_u32x2 vf[16];
   sf_u32x4 pa[2], pb[2];
@@ -423,7 +419,7 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   };
 
   // S^T of stage 0
-  sf_wait_vm_barrier<(kAhead - 1) * kCopies>();
+  sf_wait_vm_barrier<(kAhead - 1) * 4>();
   {
     sf_lds_off ka[8];
 #pragma unroll
@@ -462,15 +458,15 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
 #pragma unroll
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
     mx *= scale_log2;
-    m_hi = fmaxf(m_hi, mx);
-    resc = __ballot(mx > m_ref + kLazy) != 0;   // wave-uniform
+    resc = __ballot(mx > m_lim) != 0;   // wave-uniform
     if (resc) {
-      m_hi = fmaxf(m_hi, __shfl_xor(m_hi, 32, 64));
-      alpha = __builtin_amdgcn_exp2f(m_ref - (m_hi == -INFINITY ? 0.f : m_hi));
-      m_ref = m_hi;
+      const float m_new = fmaxf(m_ref, fmaxf(mx, __shfl_xor(mx, 32, 64)));
+      mu = m_new == -INFINITY ? 0.f : m_new;
+      alpha = __builtin_amdgcn_exp2f(m_ref - mu);
+      m_ref = m_new;
+      m_lim = m_new + kLazy;
       l_run *= alpha;
     }
-    const float mu = m_ref == -INFINITY ? 0.f : m_ref;
     float p[16];
     pv(0, 2, 4);
     pv(1, 0, 4);
@@ -520,7 +516,7 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
     for (int ks = 0; ks < 8; ++ks) ka[ks] = b0 + koff[ks];
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) va[dt] = b0 + voff[dt];
-    sf_wait_vm_barrier<(kAhead - 2) * kCopies>();
+    sf_wait_vm_barrier<(kAhead - 2) * 4>();
     issue(k + kAhead);
     step(k, sa, sb, pb, pa, ka, Int<kSlot>{}, va, Int<0>{});
     if (k + 1 == nst) {   // (workgroup-uniform) the last: its P.V follows from the b side
@@ -531,7 +527,7 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
     const sf_lds_off b1 = sf_lds_addr(ring) + ((k + 2) % kRing) * kSlot;
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) ka[ks] = b1 + koff[ks];
-    sf_wait_vm_barrier<(kAhead - 2) * kCopies>();
+    sf_wait_vm_barrier<(kAhead - 2) * 4>();
     issue(k + 1 + kAhead);
     step(k + 1, sb, sa, pa, pb, ka, Int<0>{}, va, Int<kSlot>{});
   }
@@ -581,13 +577,13 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   if (c0 >= keys.nst) return;
   const int nst = min(c.spr, keys.nst - c0);
   const int lastg = last_group(P);
-  const int32_t* const table = s.table;
-  // lane i: the page table's entry for 16-key group i & 1 of this wave's stage 32u + i / 2
-  auto load_pages = [&](int u) {
-    const int k = min(wv + 4 * (32 * u + (lane >> 1)), nst - 1);
-    return table[min(keys.key0(c0 + k) + 16 * (lane & 1), lastg) >> c.page_shift];
+  // lane i: 16-key group i & 1 of this wave's stage 32u + i / 2 (past the range: the last)
+  auto lane_group = [&](int u) {
+    return min(keys.key0(c0 + min(wv + 4 * (32 * u + (lane >> 1)), nst - 1)) + 16 * (lane & 1),
+               lastg);
   };
-  int pg = table ? load_pages(0) : 0;
+  auto load_pages = [&](int u) { return s.table ? s.table[lane_group(u) >> c.page_shift] : 0; };
+  const int pg = load_pages(0);
   const int qi = min(lane & 31, nq - 1);
   const int m = qi / G;
   const int end = row_end(m, s.rows, P, c.block), lo = row_lo(m, s.rows, P, c.window);
@@ -600,21 +596,26 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
     qf[ks] = *reinterpret_cast<const sf_u32x4*>(q + rh * kHD + 16 * ks + 8 * hf);
 
   uint8_t* mine = ring + wv * kSlot;
-  uint32_t ok[4], ov[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    ok[i] = copy_off(lane, 4 * i, false), ov[i] = copy_off(lane, 4 * i, true);
-  const Source sk = source_of(s.k, s, it.h, c.page_shift);
-  const Source sv = source_of(s.v, s, it.h, c.page_shift);
+  const uint16_t* const kb = s.k + (long long)it.h * s.head_stride;
+  const uint16_t* const vb = s.v + (long long)it.h * s.head_stride;
+  Groups groups;
+  groups.set(group_off(s, c.page_shift, pg, lane_group(0)));
   auto issue = [&](int j) {   // this wave's stage j
+    if (j > 0 && (j & 31) == 0)
+      groups.set(group_off(s, c.page_shift, load_pages(j >> 5), lane_group(j >> 5)));
     const int key0 = keys.key0(c0 + wv + 4 * j);
-    if (table && j > 0 && (j & 31) == 0) pg = load_pages(j >> 5);
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      const int g0 = min(key0 + 16 * g, lastg);
-      const int id = lane_value(pg, 2 * (j & 31) + g);
-      copy_rows<4>(sk, id, g0, 0, ok, mine + 16 * g * kRowBytes);
-      copy_rows<4>(sv, id, g0, 0, ov, mine + kHalf + 16 * g * kRowBytes);
+      const int last = min(15, P - 1 - min(key0 + 16 * g, lastg));   // of the group's rows
+      uint32_t ok[4], ov[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ok[i] = copy_off(lane, 4 * i, false, last);
+        ov[i] = copy_off(lane, 4 * i, true, last);
+      }
+      const long long at = groups.at(2 * (j & 31) + g);
+      copy_rows<4>(kb + at, ok, mine + 16 * g * kRowBytes);
+      copy_rows<4>(vb + at, ov, mine + kHalf + 16 * g * kRowBytes);
     }
   };
   if (wv < nst) issue(0);
@@ -913,18 +914,18 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
     // ---- the wave's 64 keys, stage 0, then the K operands to registers --------------------
     {
       const int lastg = last_group(P);
-      const Source src = source_of(s.k, s, it.h, c.page_shift);
-      uint32_t off[4];
+      const uint16_t* const kb = s.k + (long long)it.h * s.head_stride;
+      const int g0 = min(kw0 + 16 * (lane & 3), lastg);   // lane g: the wave's group g
+      Groups groups;
+      groups.set(group_off(s, c.page_shift, s.table ? s.table[g0 >> c.page_shift] : 0, g0));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) off[i] = copy_off(lane, 4 * i, false);
-      int id[4];
+      for (int g = 0; g < 4; ++g) {
+        uint32_t off[4];
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        id[g] = s.table ? s.table[min(kw0 + 16 * g, lastg) >> c.page_shift] : 0;
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        copy_rows<4>(src, __builtin_amdgcn_readfirstlane(id[g]), min(kw0 + 16 * g, lastg), 0, off,
-                     kmine + 16 * g * kRowBytes);
+        for (int i = 0; i < 4; ++i)
+          off[i] = copy_off(lane, 4 * i, false, min(15, P - 1 - min(kw0 + 16 * g, lastg)));
+        copy_rows<4>(kb + groups.at(g), off, kmine + 16 * g * kRowBytes);
+      }
     }
     issue(0);
     sf_wait_vm_barrier<0>();
@@ -1048,11 +1049,13 @@ __global__ __launch_bounds__(kMassKeys) void sf_window_mass_merge_kernel(
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 int make_call(const sf_kv_seq* seqs, int n_seqs, int page_size, int block, int window, int sinks,
-              int H, int Hkv, int hd, bool mass, Call& c) {
+              int H, int Hkv, int hd, float scaling, bool mass, Call& c) {
   if (!seqs) return SF_ERR_ARG;
   if (hd != kHD || H < 1 || Hkv < 1 || H % Hkv != 0 || H / Hkv > kMaxG) return SF_ERR_SHAPE;
   if (n_seqs < 1 || n_seqs > kMaxSeqs) return SF_ERR_SHAPE;
   if (block < 1 || window < 0 || sinks < 0) return SF_ERR_SHAPE;
+  // (the running maximum is the scores' before scaling)
+  if (!(scaling > 0.f && scaling < INFINITY)) return SF_ERR_ARG;
   c = Call{};
   c.n_seqs = n_seqs;
   c.page_shift = page_size > 0 ? __builtin_ctz(page_size) : 0;
@@ -1149,7 +1152,7 @@ extern "C" int sf_attn_window(const uint16_t* q, const sf_kv_seq* seqs, int n_se
                               float scaling, uint16_t* o, float* lse, void* workspace,
                               size_t workspace_bytes, void* stream) {
   Call c;
-  const int st = make_call(seqs, n_seqs, page_size, block, window, sinks, H, Hkv, hd, false, c);
+  const int st = make_call(seqs, n_seqs, page_size, block, window, sinks, H, Hkv, hd, scaling, false, c);
   if (st != SF_OK) return st;
   if (c.rows == 0) return SF_OK;
   if (!q || !o || !workspace || !aligned(q) || !aligned(o) || !aligned(workspace))
@@ -1159,29 +1162,17 @@ extern "C" int sf_attn_window(const uint16_t* q, const sf_kv_seq* seqs, int n_se
   const float scale_log2 = scaling * kLog2e;
   float* ws_o = reinterpret_cast<float*>(workspace);
   float* ws_ml = ws_o + (size_t)ranges_cap(c.rows) * c.rows * H * kHD;
-  const int G = H / Hkv;
   // sequences of up to 32 queries a kv head, then the others
   for (int few = 1; few >= 0; --few) {
-    int bq = 32, items;
-    if (few) {
-      items = plan_ranges(c, bq, 1, 32, 2 * kCUs, Cost{12, 20});
-    } else {
-      long long tiles = 0;
-      for (int i = 0; i < n_seqs; ++i)
-        if (c.s[i].rows * G > 32) tiles += tiles_of(c.s[i].rows, G, 256);
-      bq = tiles * Hkv >= kCUs ? 256 : 128;
-      items = plan_ranges(c, bq, 33, 1 << 30, bq == 256 ? kCUs : 2 * kCUs,
-                          bq == 256 ? Cost{4, 34} : Cost{6, 24});
-    }
+    const int bq = few ? 32 : kTileQ;
+    const int items = few ? plan_ranges(c, bq, 1, 32, 2 * kCUs, Cost{12, 20})
+                          : plan_ranges(c, bq, 33, 1 << 30, 2 * kCUs, Cost{6, 24});
     if (items == 0) continue;
     if (few)
       hipLaunchKernelGGL(sf_window_few_kernel, dim3(items), dim3(kThreads), 0, hs, q, c,
                          scale_log2, o, lse, ws_o, ws_ml);
-    else if (bq == 256)
-      hipLaunchKernelGGL((sf_window_tile_kernel<8>), dim3(items), dim3(512), 0, hs, q, c,
-                         scale_log2, o, lse, ws_o, ws_ml);
     else
-      hipLaunchKernelGGL((sf_window_tile_kernel<4>), dim3(items), dim3(256), 0, hs, q, c,
+      hipLaunchKernelGGL(sf_window_tile_kernel, dim3(items), dim3(kThreads), 0, hs, q, c,
                          scale_log2, o, lse, ws_o, ws_ml);
     if (c.nr > 4)
       hipLaunchKernelGGL((sf_window_merge_kernel<16>), dim3((c.rows * H + 3) / 4), dim3(kThreads),
@@ -1203,7 +1194,7 @@ extern "C" int sf_attn_key_mass(const uint16_t* q, const float* lse, const sf_kv
                                 int Hkv, int hd, float scaling, float decay, void* workspace,
                                 size_t workspace_bytes, void* stream) {
   MassCall c;
-  const int st = make_call(seqs, n_seqs, page_size, block, window, sinks, H, Hkv, hd, true, c);
+  const int st = make_call(seqs, n_seqs, page_size, block, window, sinks, H, Hkv, hd, scaling, true, c);
   if (st != SF_OK) return st;
   if (!(decay >= 0.f && decay <= 1.f)) return SF_ERR_ARG;
   if (c.rows > 0 && (!q || !lse || !aligned(q))) return SF_ERR_ARG;

@@ -358,3 +358,38 @@ def test_bad_pages_stay_inside(sim):
     others = [pg for pg in range(c.num_pages) if pg not in mapped]
     assert len(others) == 2
     assert torch.equal(c.k_pages[:, others].view(torch.int16), before[:, others].view(torch.int16))
+
+
+@pytest.mark.parametrize("what", ["window", "mass"])
+@pytest.mark.parametrize("scaling", [0.0, -0.1, math.inf, math.nan])
+def test_scaling_refused(sim, what, scaling):
+    q, ks, vs, caches = make_seqs([(3, 20)], 4, 2, 1, "cpu")
+    ws = torch.empty(1 << 23, dtype=torch.uint8)
+    batch = PagedBatch(caches, [3])
+    with pytest.raises(_lib.SpecFoldKernelError):
+        if what == "window":
+            sim.attn_window(q, batch, 0, 4, scaling, torch.empty(3, 512, dtype=BF), ws)
+        else:
+            sim.attn_key_mass(q, torch.zeros(3, 4), batch, 0, 4, scaling, [torch.zeros(2, 20)], ws)
+
+
+def test_extreme_masks(sim):
+    """Windows, sinks and blocks as large as an int holds are no mask at all."""
+    big = 2 ** 31 - 1
+    q, ks, vs, caches = make_seqs([(40, 100)], 4, 2, 1, "cpu")
+    ref = run_window(sim, q, caches, [40], 4, 1, 0, 0)
+    for window, sinks in ((big, 0), (big, big), (1, big), (0, big)):
+        got = run_window(sim, q, caches, [40], 4, 1, window, sinks)
+        assert torch.equal(ref[0], got[0]) and torch.equal(ref[1], got[1])
+    ref = run_window(sim, q, caches, [40], 4, 40, 0, 0)
+    got = run_window(sim, q, caches, [40], 4, big, 0, 0)
+    assert torch.equal(ref[0], got[0]) and torch.equal(ref[1], got[1])
+    for window, sinks, block in ((big, 0, 1), (1, big, 1), (0, big, big)):
+        ws = torch.zeros(sim.attn_key_mass_workspace_bytes(100, 2), dtype=torch.uint8)
+        outs = []
+        for kw in (dict(block=block), dict(block=block, window=window, sinks=sinks)):
+            out = [torch.zeros(2, 100)]
+            sim.attn_key_mass(q, ref[1].contiguous(), PagedBatch(caches, [40]), 0, 4, HD ** -0.5,
+                              out, ws, **kw)
+            outs.append(out[0])
+        assert torch.equal(*outs)

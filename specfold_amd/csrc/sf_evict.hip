@@ -5,11 +5,15 @@
 // k = keep - sinks - recent others with the largest mass, equal ones by the lower index.
 //  * select: one workgroup per (layer, kv head).  The masses are mapped to unsigned
 //    integers of the same order and stay in registers; the k-th largest value is built
-//    bit by bit from the top (how many are >= the candidate), exact and without atomics;
-//    two ballot scans number the ties and the kept keys in index order.
-//  * move: the kept rows to slots 0 .. keep - 1, ascending.  Slot j takes a row from a
-//    slot >= j, so a workgroup that goes up the slots, every row of a tile read before
-//    the tile is written, may move in place.
+//    two bits at a time from the top by counting the keys that are not below each
+//    candidate (ballots; exact, no atomics), until the count is k or no bit is left; two
+//    ballot scans number the ties and the kept keys in index order.  Bound by the steps'
+//    barriers (about 0.5 us each).
+//  * move: the kept rows to slots 0 .. keep - 1, ascending, bound by reading and writing
+//    them once.  Into another cache every 128 rows are a workgroup's.  In place slot j
+//    takes a row from a slot >= j, so a workgroup goes up the slots of its (layer, kv
+//    head) alone: a tile is written when all of its rows have been read, and the rows of
+//    the tile behind it, which no write of this one reaches, are on their way.
 #include "sf_common.h"
 
 namespace {
@@ -26,22 +30,13 @@ SF_DEV uint32_t order_of(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-SF_DEV int block_sum(int v, int* s_red) {
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  int t = 0;
-  for (int w = 0; w < kSelWaves; ++w) t += s_red[w];
-  return t;
-}
-
 template <int PER>   // keys of a thread: t = i * 1024 + tid
 __global__ __launch_bounds__(kSelThreads) void sf_evict_select_kernel(
     const float* mass, long long mass_layer, long long mass_head, int Hkv, int P, int sinks,
     int recent, int keep, int32_t* __restrict__ kept, float* mass_out, long long out_layer,
     long long out_head, int zero_to) {
-  __shared__ int s_red[kSelWaves];
+  __shared__ int s_red[2][64];
+  __shared__ int s_above[kSelWaves];
   __shared__ int s_cnt[PER * kSelWaves];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int l = blockIdx.x / Hkv, h = blockIdx.x - l * Hkv;
@@ -55,14 +50,32 @@ __global__ __launch_bounds__(kSelThreads) void sf_evict_select_kernel(
     key[i] = t >= sinks && t < last ? order_of(in[t]) : 0u;
   }
   const int need = keep - sinks - recent;   // <= last - sinks
-  uint32_t thr = 0;                         // the need-th largest
+  // thr: the need-th largest, or (exact) a bound that just the `need` largest reach
+  uint32_t thr = 0;
+  bool exact = false;
   if (need > 0) {
-    for (int b = 31; b >= 0; --b) {
-      const uint32_t cand = thr | (1u << b);
-      int n = 0;
+#pragma unroll 1
+    for (int sh = 30; sh >= 0 && !exact; sh -= 2) {   // workgroup-uniform
+      int n[3];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) n += key[i] >= cand ? 1 : 0;
-      if (block_sum(n, s_red) >= need) thr = cand;
+      for (int d = 0; d < 3; ++d) {
+        const uint32_t cand = thr | ((uint32_t)(d + 1) << sh);
+        n[d] = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) n[d] += __popcll(__ballot(key[i] >= cand));
+      }
+      int* red = s_red[(sh >> 1) & 1];   // (two in turn: one barrier a step)
+      if (lane < 3) red[wv * 4 + lane] = lane == 0 ? n[0] : lane == 1 ? n[1] : n[2];
+      __syncthreads();
+      // lane 4w + d: wave w's count of candidate d + 1; then the sums over the waves
+      int t = (lane & 3) < 3 ? red[lane] : 0;
+#pragma unroll
+      for (int o = 4; o <= 32; o <<= 1) t += __shfl_xor(t, o, 64);
+      const int digit = __popcll(__ballot(t >= need && (lane & 3) < 3) & 7ull);   // falling counts
+      if (digit > 0) {
+        thr |= (uint32_t)digit << sh;
+        exact = __shfl(t, digit - 1, 64) == need;
+      }
     }
   }
   int above = 0;
@@ -71,11 +84,12 @@ __global__ __launch_bounds__(kSelThreads) void sf_evict_select_kernel(
   for (int i = 0; i < PER; ++i) {
     const int t = i * kSelThreads + tid;
     const bool mid = t >= sinks && t < last;
-    if (t < P && (!mid || (need > 0 && key[i] > thr))) keeps |= 1u << i;
-    if (mid && need > 0 && key[i] == thr) equal |= 1u << i;
-    above += mid && need > 0 && key[i] > thr ? 1 : 0;
+    const bool in_it = mid & (need > 0);
+    const bool over = in_it & (exact ? key[i] >= thr : key[i] > thr);
+    if (t < P && (!mid || over)) keeps |= 1u << i;
+    if (in_it && !exact && key[i] == thr) equal |= 1u << i;
+    above += over ? 1 : 0;
   }
-  const int ties = need - block_sum(above, s_red);   // of the equal ones the first `ties`
   // index-order numbering of the flagged keys: s_cnt holds, for each 64 of them, how
   // many are flagged in front
   auto scan = [&](uint32_t bits) {
@@ -86,23 +100,39 @@ __global__ __launch_bounds__(kSelThreads) void sf_evict_select_kernel(
       if (lane == 0) s_cnt[i * kSelWaves + wv] = __popcll(b);
     }
     __syncthreads();
-    if (tid == 0) {
-      int at = 0;
-      for (int j = 0; j < PER * kSelWaves; ++j) {
-        const int n = s_cnt[j];
-        s_cnt[j] = at;
-        at += n;
+    if (wv == 0) {   // lane x: entries x PER / 4 ..
+      constexpr int kE = PER / 4;
+      int e[kE], sum = 0;
+#pragma unroll
+      for (int i = 0; i < kE; ++i) {
+        e[i] = sum;
+        sum += s_cnt[lane * kE + i];
       }
+      int at = sum;
+#pragma unroll
+      for (int o = 1; o <= 32; o <<= 1) {
+        const int up = __shfl(at, lane >= o ? lane - o : lane, 64);
+        at += lane >= o ? up : 0;
+      }
+      at -= sum;
+#pragma unroll
+      for (int i = 0; i < kE; ++i) s_cnt[lane * kE + i] = at + e[i];
     }
     __syncthreads();
   };
   const unsigned long long below = (1ull << lane) - 1;
-  scan(equal);
+  if (need > 0 && !exact) {   // of the equal ones the first need - (those above)
+    for (int o = 32; o >= 1; o >>= 1) above += __shfl_xor(above, o, 64);
+    if (lane == 0) s_above[wv] = above;
+    scan(equal);
+    int ties = need;
+    for (int w = 0; w < kSelWaves; ++w) ties -= s_above[w];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const unsigned long long b = __ballot(equal >> i & 1u);
-    const int rank = s_cnt[i * kSelWaves + wv] + __popcll(b & below);
-    if ((equal >> i & 1u) && rank < ties) keeps |= 1u << i;
+    for (int i = 0; i < PER; ++i) {
+      const unsigned long long b = __ballot(equal >> i & 1u);
+      const int rank = s_cnt[i * kSelWaves + wv] + __popcll(b & below);
+      if ((equal >> i & 1u) && rank < ties) keeps |= 1u << i;
+    }
   }
   scan(keeps);
   int32_t* kp = kept + (size_t)blockIdx.x * keep;
@@ -143,33 +173,68 @@ SF_DEV long long slot_off(const Pages& p, int l, int h, int t, bool& ok) {
 }
 
 constexpr int kMoveThreads = 256;
-constexpr int kMoveRows = 8;   // rows of a thread in a tile: 16 * 8 rows a tile
-__global__ __launch_bounds__(kMoveThreads) void sf_evict_move_kernel(
+constexpr int kMoveRows = 8;   // 16-byte units of a thread in a tile
+
+// Into another cache: 16 threads a row, 128 rows a workgroup.
+__global__ __launch_bounds__(kMoveThreads) void sf_evict_copy_kernel(
     Pages fk, Pages fv, Pages tk, Pages tv, const int32_t* __restrict__ kept, int Hkv, int keep) {
-  const int l = blockIdx.x / Hkv, h = blockIdx.x - l * Hkv;
+  const int tiles = (keep + 16 * kMoveRows - 1) / (16 * kMoveRows);
+  const int lh = blockIdx.x / tiles, j0 = (blockIdx.x - lh * tiles) * 16 * kMoveRows;
+  const int l = lh / Hkv, h = lh - l * Hkv;
   const Pages from = blockIdx.y ? fv : fk, to = blockIdx.y ? tv : tk;
+  const int32_t* kp = kept + (size_t)lh * keep;
+  const int unit = threadIdx.x & 15, r = j0 + (threadIdx.x >> 4);
+  sf_u32x4 w[kMoveRows];
+#pragma unroll
+  for (int i = 0; i < kMoveRows; ++i) {
+    bool ok;
+    const long long at = slot_off(from, l, h, kp[min(r + 16 * i, keep - 1)], ok);
+    w[i] = sf_stream_load16(from.base + at + unit * 8);
+  }
+#pragma unroll
+  for (int i = 0; i < kMoveRows; ++i) {
+    bool ok;
+    const long long at = slot_off(to, l, h, min(r + 16 * i, keep - 1), ok);
+    if (r + 16 * i < keep && ok)
+      sf_handoff_store(reinterpret_cast<sf_u32x4*>(to.base + at + unit * 8), w[i]);
+  }
+}
+
+// In place: 8 threads a half row (64 dims), 256 rows a tile; blockIdx.y: K or V, its half.
+__global__ __launch_bounds__(kMoveThreads) void sf_evict_move_kernel(
+    Pages pk, Pages pv, const int32_t* __restrict__ kept, int Hkv, int keep) {
+  constexpr int kTile = 32 * kMoveRows;
+  const int l = blockIdx.x / Hkv, h = blockIdx.x - l * Hkv;
+  const Pages pg = blockIdx.y >> 1 ? pv : pk;
   const int32_t* kp = kept + (size_t)blockIdx.x * keep;
-  const int unit = threadIdx.x & 15, r = threadIdx.x >> 4;
-  for (int j0 = 0; j0 < keep; j0 += 16 * kMoveRows) {
-    sf_u32x4 w[kMoveRows];
+  const int dim = 64 * (blockIdx.y & 1) + 8 * (threadIdx.x & 7), r = threadIdx.x >> 3;
+  sf_u32x4 cur[kMoveRows], next[kMoveRows];
+  auto load = [&](int j0, sf_u32x4 (&w)[kMoveRows]) {
 #pragma unroll
     for (int i = 0; i < kMoveRows; ++i) {
-      const int j = min(j0 + 16 * i + r, keep - 1);
       bool ok;
-      const long long at = slot_off(from, l, h, kp[j], ok);
-      w[i] = *reinterpret_cast<const sf_u32x4*>(from.base + at + unit * 8);
+      const long long at = slot_off(pg, l, h, kp[min(j0 + 32 * i + r, keep - 1)], ok);
+      w[i] = *reinterpret_cast<const sf_u32x4*>(pg.base + at + dim);
     }
+  };
+  auto store = [&](int j0, sf_u32x4 (&w)[kMoveRows]) {
 #pragma unroll
-    for (int i = 0; i < kMoveRows; ++i) sf_pin(w[i]);
-    sf_wait_vm_loads();
-    __syncthreads();
+    for (int i = 0; i < kMoveRows; ++i) sf_pin(w[i]);   // (this thread's rows of the tile are here)
+    __syncthreads();                                    // and everyone's
 #pragma unroll
     for (int i = 0; i < kMoveRows; ++i) {
-      const int j = j0 + 16 * i + r;
+      const int j = j0 + 32 * i + r;
       bool ok;
-      const long long at = slot_off(to, l, h, min(j, keep - 1), ok);
-      if (j < keep && ok) *reinterpret_cast<sf_u32x4*>(to.base + at + unit * 8) = w[i];
+      const long long at = slot_off(pg, l, h, min(j, keep - 1), ok);
+      if (j < keep && ok) *reinterpret_cast<sf_u32x4*>(pg.base + at + dim) = w[i];
     }
+  };
+  load(0, cur);
+  for (int j0 = 0; j0 < keep; j0 += 2 * kTile) {   // (tiles past the end: nothing is written)
+    load(j0 + kTile, next);
+    store(j0, cur);
+    load(j0 + 2 * kTile, cur);
+    store(j0 + kTile, next);
   }
 }
 
@@ -200,6 +265,12 @@ extern "C" int sf_kv_evict(const float* mass, long long mass_layer, long long ma
   if (st != SF_OK) return st;
   if (mass_out == mass && (mass_out_layer != mass_layer || mass_out_head != mass_head))
     return SF_ERR_ARG;
+  // the same pool through the same table: the same mapping, in place
+  const bool in_place = from->k == to->k && from->page_table == to->page_table;
+  if (in_place && (from->v != to->v || from->layer_stride != to->layer_stride ||
+                   from->page_stride != to->page_stride || from->head_stride != to->head_stride ||
+                   from->page_size != to->page_size))
+    return SF_ERR_ARG;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define SF_EVICT_SELECT(PER)                                                                    \
   hipLaunchKernelGGL((sf_evict_select_kernel<PER>), dim3(layers * Hkv), dim3(kSelThreads), 0, s, \
@@ -213,8 +284,14 @@ extern "C" int sf_kv_evict(const float* mass, long long mass_layer, long long ma
     return Pages{base, p->page_table, p->layer_stride, p->page_stride, p->head_stride,
                  p->page_size, p->pages};
   };
-  hipLaunchKernelGGL(sf_evict_move_kernel, dim3(layers * Hkv, 2), dim3(kMoveThreads), 0, s,
-                     pages(from, from->k), pages(from, from->v), pages(to, to->k),
-                     pages(to, to->v), kept, Hkv, keep);
+  if (in_place) {
+    hipLaunchKernelGGL(sf_evict_move_kernel, dim3(layers * Hkv, 4), dim3(kMoveThreads), 0, s,
+                       pages(to, to->k), pages(to, to->v), kept, Hkv, keep);
+  } else {
+    const int tiles = (keep + 16 * kMoveRows - 1) / (16 * kMoveRows);
+    hipLaunchKernelGGL(sf_evict_copy_kernel, dim3(layers * Hkv * tiles, 2), dim3(kMoveThreads), 0,
+                       s, pages(from, from->k), pages(from, from->v), pages(to, to->k),
+                       pages(to, to->v), kept, Hkv, keep);
+  }
   return sf_launch_status();
 }

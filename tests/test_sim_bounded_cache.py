@@ -292,6 +292,7 @@ def _evict(lib, **over):
     (dict(recent=-1), SHAPE), (dict(sinks=30, recent=3), SHAPE), (dict(sinks=33), SHAPE),
     (dict(page_size=24), SHAPE), (dict(to_page_size=8), SHAPE), (dict(pages=3), SHAPE),
     (dict(to_pages=1), SHAPE), (dict(page_stride=4), SHAPE), (dict(to_layer_stride=7), SHAPE),
+    (dict(to_v=4096 * 5), ARG), (dict(to_head_stride=4096), ARG), (dict(to_page_size=32), ARG),
     (dict(mass_out=4096, oml=128, omh=63), ARG)])
 def test_evict_refusals(over, code):
     assert _evict(_lib.load(), **over) == code

@@ -9,7 +9,6 @@ pointers and the current HIP stream.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from pathlib import Path
 from typing import Optional
@@ -150,8 +149,10 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _stream(stream=None):
-    s = torch.cuda.current_stream() if stream is None else stream
-    return ctypes.c_void_p(s.cuda_stream)
+    if stream is not None:
+        return ctypes.c_void_p(stream.cuda_stream)
+    # the current stream's handle without a Stream object (which takes 3 us)
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, numel: Optional[int] = None,
@@ -469,17 +470,17 @@ def attn_key_mass_workspace_bytes(keys: int, Hkv: int) -> int:
     return int(load().sf_attn_key_mass_workspace_bytes(keys, Hkv))
 
 
-@contextlib.contextmanager
-def _on(t: torch.Tensor, **others):
-    """The device of ``t`` current, the other tensors (None allowed) checked to be on it."""
-    for nm, o in others.items():
-        if o is not None and o.device != t.device:
-            raise ValueError(f"{nm}: on {o.device}, expected {t.device}")
-    if t.device.type != "cuda" or t.device.index == torch.cuda.current_device():
-        yield
-    else:
-        with torch.cuda.device(t.device):
-            yield
+def _on_device(fn, t: torch.Tensor, others, stream, *args):
+    """fn(*args, stream handle) with the device of ``t`` current; the (name, tensor) pairs
+    ``others`` (None allowed) have to be on it."""
+    dev = t.device
+    for nm, o in others:
+        if o is not None and o.device != dev:
+            raise ValueError(f"{nm}: on {o.device}, expected {dev}")
+    if dev.type != "cuda" or dev.index == torch.cuda.current_device():
+        return fn(*args, _stream(stream))
+    with torch.cuda.device(dev):
+        return fn(*args, _stream(stream))
 
 
 def attn_window(q, batch, li, H, scaling, o, workspace, lse=None, block: int = 1, window: int = 0,
@@ -496,11 +497,17 @@ def attn_window(q, batch, li, H, scaling, o, workspace, lse=None, block: int = 1
         _need(lse, "lse", torch.float32, min_numel=rows * H, align=4)
     _need(workspace, "workspace", torch.uint8, min_numel=attn_window_workspace_bytes(rows, H))
     seqs = batch.seqs(li)
-    with _on(q, o=o, lse=lse, workspace=workspace, caches=batch):
-        st = load().sf_attn_window(_ptr(q), seqs, len(seqs), batch.page_size, block, window, sinks,
-                                   H, batch.Hkv, hd, float(scaling), _ptr(o), _ptr(lse),
-                                   _ptr(workspace), workspace.numel(), _stream(stream))
+    st = _on_device(load().sf_attn_window, q,
+                    (("o", o), ("lse", lse), ("workspace", workspace), ("caches", batch)), stream,
+                    q.data_ptr(), seqs, len(seqs), batch.page_size, block, window, sinks, H,
+                    batch.Hkv, hd, scaling, o.data_ptr(), None if lse is None else lse.data_ptr(),
+                    workspace.data_ptr(), workspace.numel())
     _check(st, "sf_attn_window")
+
+
+def _bad_mass(name, t, Hkv, n, dev) -> ValueError:
+    return ValueError(f"{name}: expected float32 [{Hkv}, >= {n}] with contiguous rows on {dev}, "
+                      f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def attn_key_mass(q, lse, batch, li, H, scaling, mass, workspace, mass_in=None, decay: float = 1.0,
@@ -513,30 +520,32 @@ def attn_key_mass(q, lse, batch, li, H, scaling, mass, workspace, mass_in=None, 
     _need(q, "q", torch.bfloat16, min_numel=rows * H * hd)
     _need(lse, "lse", torch.float32, min_numel=rows * H, align=4)
     seqs = batch.seqs(li)
-    total = sum(s.length for s in seqs)
     _need(workspace, "workspace", torch.uint8,
-          min_numel=attn_key_mass_workspace_bytes(total, batch.Hkv))
-    for name, ts in (("mass", mass), ("mass_in", mass_in)):
-        if ts is None:
-            continue
-        if len(ts) != len(seqs):
-            raise ValueError(f"{name}: one tensor per sequence, got {len(ts)} for {len(seqs)}")
-        for s, t in zip(seqs, ts):
-            if t.dtype != torch.float32 or t.dim() != 2 or t.shape[0] != batch.Hkv or \
-                    t.shape[1] < s.length or t.stride(1) != 1:
-                raise ValueError(f"{name}: expected float32 [{batch.Hkv}, >= {s.length}] with "
-                                 f"contiguous rows, got {t.dtype} {tuple(t.shape)}")
-            if t.device != q.device:
-                raise ValueError(f"{name}: on {t.device}, expected {q.device}")
-            if name == "mass":
-                s.mass_out, s.mass_out_stride = t.data_ptr(), t.stride(0)
-                s.mass_in, s.mass_in_stride = None, 0
-            else:
-                s.mass_in, s.mass_in_stride = t.data_ptr(), t.stride(0)
-    with _on(q, lse=lse, workspace=workspace, caches=batch):
-        st = load().sf_attn_key_mass(_ptr(q), _ptr(lse), seqs, len(seqs), batch.page_size, block,
-                                     window, sinks, H, batch.Hkv, hd, float(scaling), float(decay),
-                                     _ptr(workspace), workspace.numel(), _stream(stream))
+          min_numel=attn_key_mass_workspace_bytes(batch.num_keys, batch.Hkv))
+    if len(mass) != len(seqs) or (mass_in is not None and len(mass_in) != len(seqs)):
+        raise ValueError(f"mass, mass_in: one tensor per sequence ({len(seqs)})")
+    dev, Hkv = q.device, batch.Hkv
+    for i, s in enumerate(seqs):
+        t, u = mass[i], None if mass_in is None else mass_in[i]
+        stride, n = t.stride(), s.length
+        if t.dtype is not torch.float32 or t.dim() != 2 or t.shape[0] != Hkv or \
+                t.shape[1] < n or stride[1] != 1 or t.device != dev:
+            raise _bad_mass("mass", t, Hkv, n, dev)
+        s.mass_out, s.mass_out_stride = t.data_ptr(), stride[0]
+        if u is t:
+            s.mass_in, s.mass_in_stride = t.data_ptr(), stride[0]
+        elif u is None:
+            s.mass_in = None
+        else:
+            stride = u.stride()
+            if u.dtype is not torch.float32 or u.dim() != 2 or u.shape[0] != Hkv or \
+                    u.shape[1] < n or stride[1] != 1 or u.device != dev:
+                raise _bad_mass("mass_in", u, Hkv, n, dev)
+            s.mass_in, s.mass_in_stride = u.data_ptr(), stride[0]
+    st = _on_device(load().sf_attn_key_mass, q,
+                    (("lse", lse), ("workspace", workspace), ("caches", batch)), stream,
+                    q.data_ptr(), lse.data_ptr(), seqs, len(seqs), batch.page_size, block, window,
+                    sinks, H, Hkv, hd, scaling, decay, workspace.data_ptr(), workspace.numel())
     _check(st, "sf_attn_key_mass")
 
 
@@ -569,12 +578,14 @@ def kv_evict(mass, length: int, keep: int, sinks: int, recent: int, src, dst, ke
         pages.append(KVPages(c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.page_table.data_ptr(),
                              c.k_pages.stride(0), c.k_pages.stride(1), c.k_pages.stride(2),
                              c.page_size, c.num_pages))
-    with _on(mass, kept=kept, mass_out=mass_out, src=src.k_pages, dst=dst.k_pages):
-        st = load().sf_kv_evict(
-            _ptr(mass), mass.stride(0), mass.stride(1), L, Hkv, hd, length, sinks, recent, keep,
-            ctypes.byref(pages[0]), ctypes.byref(pages[1]), _ptr(kept), _ptr(mass_out),
-            0 if mass_out is None else mass_out.stride(0),
-            0 if mass_out is None else mass_out.stride(1), _stream(stream))
+    none = mass_out is None
+    st = _on_device(load().sf_kv_evict, mass,
+                    (("kept", kept), ("mass_out", mass_out), ("src", src.k_pages),
+                     ("dst", dst.k_pages)), stream,
+                    mass.data_ptr(), mass.stride(0), mass.stride(1), L, Hkv, hd, length, sinks,
+                    recent, keep, ctypes.byref(pages[0]), ctypes.byref(pages[1]), kept.data_ptr(),
+                    None if none else mass_out.data_ptr(), 0 if none else mass_out.stride(0),
+                    0 if none else mass_out.stride(1))
     _check(st, "sf_kv_evict")
 
 

@@ -1099,12 +1099,12 @@ int make_call(const sf_kv_seq* seqs, int n_seqs, int page_size, int block, int w
 struct Cost {
   int one, many;   // stages' worth of an item's fixed part, in one range / several
 };
-void plan_spread(Call& c, long long work, int longest, int cap, int slots, Cost fix) {
+void plan_spread(Call& c, long long work, int longest, int cap, int slots, Cost fix, int unit) {
   double best = 0;
   for (int nr = 1; nr <= cap && nr <= longest; ++nr) {
-    const int spr = (longest + nr - 1) / nr;
+    const int spr = ((longest + nr - 1) / nr + unit - 1) / unit * unit;
     const double items = c.Hkv * (nr == 1 ? (double)c.tiles : (double)work / spr + 0.5 * c.tiles);
-    const double one = spr + (nr == 1 ? fix.one : fix.many);
+    const double one = spr + (nr == 1 ? fix.one : fix.many + fix.many * (nr / 16) / 4);
     const double all = (c.Hkv * (double)work + items * (one - spr)) / slots;
     const double cost = items <= slots ? one : all + 0.5 * one;
     if (nr == 1 || cost < best) {
@@ -1116,7 +1116,7 @@ void plan_spread(Call& c, long long work, int longest, int cap, int slots, Cost 
 }
 
 // The tiles of the sequences with least to most queries a kv head, and their ranges.
-int plan_ranges(Call& c, int bq, int least, int most, int slots, Cost fix) {
+int plan_ranges(Call& c, int bq, int least, int most, int slots, Cost fix, int unit) {
   const int G = c.H / c.Hkv;
   long long work = 0;
   int longest = 0;
@@ -1135,7 +1135,7 @@ int plan_ranges(Call& c, int bq, int least, int most, int slots, Cost fix) {
     }
   }
   if (c.tiles == 0) return 0;
-  plan_spread(c, work, longest, ranges_cap(c.rows), slots, fix);
+  plan_spread(c, work, longest, ranges_cap(c.rows), slots, fix, unit);
   return c.tiles * c.nr * c.Hkv;
 }
 
@@ -1162,11 +1162,26 @@ extern "C" int sf_attn_window(const uint16_t* q, const sf_kv_seq* seqs, int n_se
   const float scale_log2 = scaling * kLog2e;
   float* ws_o = reinterpret_cast<float*>(workspace);
   float* ws_ml = ws_o + (size_t)ranges_cap(c.rows) * c.rows * H * kHD;
-  // sequences of up to 32 queries a kv head, then the others
+  // Sequences of up to 32 queries a kv head, then the others.  Beside others, short ones go
+  // along in tiles that they leave mostly empty: a launch of their own takes about 8 us,
+  // in which the CUs walk some 3500 stages of such tiles (a call of 2, 26, 30 and 32 rows
+  // over 2000 keys, 28 / 4 heads: 33 us in two launches, 22 in one).
+  const int G = H / Hkv;
+  long long few_stages = 0;
+  bool others = false;
+  for (int i = 0; i < n_seqs; ++i) {
+    const Seq& x = c.s[i];
+    if (x.rows * G > 32)
+      others = true;
+    else if (x.rows > 0)
+      few_stages += tile_keys(0, x.rows - 1, x.rows, x.length, block, window, sinks).nst;
+  }
+  const int few_most = others && few_stages * Hkv < 3500 ? 0 : 32;
   for (int few = 1; few >= 0; --few) {
     const int bq = few ? 32 : kTileQ;
-    const int items = few ? plan_ranges(c, bq, 1, 32, 2 * kCUs, Cost{12, 20})
-                          : plan_ranges(c, bq, 33, 1 << 30, 2 * kCUs, Cost{6, 24});
+    const int items =
+        few ? plan_ranges(c, bq, 1, few_most, 2 * kCUs, Cost{12, 20}, 4)
+            : plan_ranges(c, bq, few_most + 1, 1 << 30, 2 * kCUs, Cost{6, 24}, 1);
     if (items == 0) continue;
     if (few)
       hipLaunchKernelGGL(sf_window_few_kernel, dim3(items), dim3(kThreads), 0, hs, q, c,
@@ -1223,7 +1238,7 @@ extern "C" int sf_attn_key_mass(const uint16_t* q, const float* lse, const sf_kv
   if (c.keys == 0) return SF_OK;
   if (!workspace || !aligned(workspace)) return SF_ERR_ARG;
   if (workspace_bytes < sf_attn_key_mass_workspace_bytes(c.keys, Hkv)) return SF_ERR_WORKSPACE;
-  plan_spread(c, work, longest, kMassRanges, 2 * kCUs, Cost{6, 10});
+  plan_spread(c, work, longest, kMassRanges, 2 * kCUs, Cost{6, 10}, 1);
   hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
   float* ws = reinterpret_cast<float*>(workspace);
   hipLaunchKernelGGL(sf_window_mass_kernel, dim3(c.tiles * c.nr * Hkv), dim3(kThreads), 0, hs, q,

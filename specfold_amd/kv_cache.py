@@ -181,7 +181,7 @@ class PagedBatch:
     sequence behind the other, whose K/V are the last keys of ``caches[s]`` (PagedKVCache
     or ContiguousMirror; alike in kv heads, head size and page size).  Lengths are read
     from the caches at every call.  ``ahead``: the rows are appended (append_rows) but not
-    yet counted (advance)."""
+    yet counted (advance).  For one host thread at a time: the calls fill its arrays."""
 
     def __init__(self, caches: Sequence, rows: Sequence[int], ahead: bool = False):
         if not caches or len(caches) != len(rows):
@@ -205,7 +205,7 @@ class PagedBatch:
 
     def seqs(self, li: int):
         """Layer li's sf_kv_seq array at the caches' present lengths."""
-        arr, arr_views = self._layers.get(li, (None, []))
+        arr, views, lengths = self._layers.get(li, (None, [], None))
         if arr is None:
             arr = (_lib.KVSeq * len(self.caches))()
             for s, c in zip(arr, self.caches):
@@ -216,12 +216,16 @@ class PagedBatch:
                 s.page_table = None if vw.page_table is None else vw.page_table.data_ptr()
                 s.page_stride, s.head_stride = vw.page_stride, vw.head_stride
                 s.pages = 0 if vw.page_table is None else vw.k.shape[0]
-                arr_views.append(vw)
-            self._layers[li] = arr, arr_views    # (the views keep the buffers)
-        for s, c, n in zip(arr, self.caches, self.rows):
-            s.length, s.rows = c.length + (n if self.ahead else 0), n
-            if s.length > c.capacity:
-                raise ValueError(f"{s.length} keys exceed the cache's capacity {c.capacity}")
+                views.append(vw)     # (keep the buffers)
+            lengths = None
+        now = [c.length for c in self.caches]
+        if now != lengths:      # the array holds other lengths than the caches
+            for s, c, n, length in zip(arr, self.caches, self.rows, now):
+                s.rows, s.length = n, length + (n if self.ahead else 0)
+                if s.length > c.capacity:
+                    raise ValueError(f"{s.length} keys exceed the cache's capacity {c.capacity}")
+            self._layers[li] = arr, views, now
+        self.num_keys = sum(now) + (self.num_rows if self.ahead else 0)
         return arr
 
 

@@ -517,7 +517,7 @@ typedef struct sf_kv_seq {
  * them.  Results do not depend on the order of pages or of workgroups.
  * workspace: sf_attn_window_workspace_bytes(rows, H) bytes, 16-byte aligned; calls that
  * share one must not overlap (two captured graphs that may replay at once need two).
- * Limits: hd == 128, H % Hkv == 0, H/Hkv <= 16, 1 <= n_seqs <= 32, 0 <= rows <= length
+ * Limits: hd == 128, H % Hkv == 0, H/Hkv <= 16, H <= 256, 1 <= n_seqs <= 32, 0 <= rows <= length
  * <= 32768 (each sequence), block >= 1, window >= 0, sinks >= 0, scaling positive and
  * finite; page_size 16, 32, 64 or
  * 128 where a page_table is given; strides multiples of 8 elements, 16-byte aligned

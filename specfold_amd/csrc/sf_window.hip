@@ -28,6 +28,7 @@ constexpr int kHD = 128;
 constexpr int kMaxSeqs = 32;
 constexpr int kMaxKeys = 32768;
 constexpr int kMaxG = 16;
+constexpr int kMaxH = 256;   // (a sequence's rows of q: 32-bit byte offsets)
 constexpr int kThreads = 256;
 constexpr int kCUs = 256;
 constexpr int kTileQ = 128;   // queries of a tile
@@ -293,17 +294,22 @@ SF_DEV void write_partial(const sf_f32x16 (&acc)[4], float m, float l, int hf, f
 }
 
 // Work item of block b: the kv head fastest (blocks go round robin over the 8 XCDs, so
-// with 1, 2, 4 or 8 kv heads a head stays on its XCDs and their L2), then the range, then
-// the sequences' tiles, the last tile of a sequence (the most keys) first.
+// with 1, 2, 4 or 8 kv heads a head stays on its XCDs and their L2).  Then the sequences'
+// tiles, the last tile of a sequence (the most keys) first, then the range: blocks of
+// ranges that a tile does not have end at once, and stand behind those that work
+// (INNER = false; 1494 causal rows of 12 / 2 heads: 67 us with the ranges inside, 53).
+// INNER: the ranges of a tile side by side, for the few-query kernel (8 tokens over 8
+// sequences of unlike lengths: 31 us, 38 with the ranges outside).
 struct Item {
   int si, tile, r, h;
 };
+template <bool INNER>
 SF_DEV Item find_item(const Call& c) {
   Item it;
   it.h = blockIdx.x % c.Hkv;
   const int rest = blockIdx.x / c.Hkv;
-  it.r = rest % c.nr;
-  const int tt = rest / c.nr;
+  it.r = INNER ? rest % c.nr : rest / c.tiles;
+  const int tt = INNER ? rest / c.nr : rest % c.tiles;
   it.si = 0;
   while (tt >= c.s[it.si].tile0 + c.s[it.si].tiles) ++it.si;
   it.tile = c.s[it.si].tiles - 1 - (tt - c.s[it.si].tile0);
@@ -326,7 +332,7 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
                       uint16_t* __restrict__ o, float* __restrict__ lse, float* __restrict__ ws_o,
                       float* __restrict__ ws_ml) {
   __shared__ __attribute__((aligned(16))) uint8_t ring[kRing * kSlot];
-  const Item it = find_item(c);
+  const Item it = find_item<false>(c);
   const Seq& s = c.s[it.si];
   const int lane = threadIdx.x & 63, hf = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // wave-uniform
@@ -368,25 +374,36 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   uint32_t off[4], off_last[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    off[i] = copy_off(lane, 4 * i, is_v, 15);
-    off_last[i] = copy_off(lane, 4 * i, is_v, P - 1 - lastg);
+    off[i] = 2 * copy_off(lane, 4 * i, is_v, 15);   // (bytes)
+    off_last[i] = 2 * copy_off(lane, 4 * i, is_v, P - 1 - lastg);
   }
   uint8_t* const dst = ring + (is_v ? kHalf : 0) + 16 * grp * kRowBytes;
   const int k_last = keys.stage_of(lastg - 16 * grp) - c0;   // from this stage on
   Groups groups;   // of the 32 stages being copied
-  auto issue = [&](int k) {   // past the range: its last stage again
+  // The copies of a stage go out one at a time between the parts of a step: right behind
+  // the barrier the sixteen of a workgroup queue up and hold their waves.
+  const char* from = nullptr;   // the stage being copied
+  uint8_t* to = dst;
+  bool last = false;
+  auto aim = [&](int k) {   // past the range: its last stage again
     if ((k & 31) == 0) {
       groups.set(group_off(s, c.page_shift, pg_next, lane_group(k >> 5)));
       pg_next = load_pages((k >> 5) + 1);
     }
-    const bool last = k >= k_last;   // wave-uniform
-    uint32_t of[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) of[i] = last ? off_last[i] : off[i];
-    copy_rows<4>(base + groups.at(2 * (k & 31) + grp), of, dst + (k % kRing) * kSlot);
+    last = k >= k_last;   // wave-uniform
+    from = reinterpret_cast<const char*>(base + groups.at(2 * (k & 31) + grp));
+    to = dst + (k % kRing) * kSlot;
+  };
+  auto copy = [&](int i) {
+    sf_lds_dma16(from + (last ? off_last[i] : off[i]), to + 4 * i * kRowBytes);
+    __builtin_amdgcn_sched_barrier(0);
   };
 #pragma unroll 1
-  for (int k = 0; k < kAhead; ++k) issue(k);
+  for (int k = 0; k < kAhead; ++k) {
+    aim(k);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) copy(i);
+  }
 
   uint32_t koff[8], voff[4];
 #pragma unroll
@@ -453,6 +470,7 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
         if (dt >= d0 && dt < d1)
           acc[dt] = mfma32(v_operand(vf, kk, dt), sf_as_bf16x8(pp[kk]), acc[dt]);
     };
+    copy(0);
     pv(0, 0, 2);
     float mx = sc[0];
 #pragma unroll
@@ -468,6 +486,7 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
       l_run *= alpha;
     }
     float p[16];
+    copy(1);
     pv(0, 2, 4);
     pv(1, 0, 4);
 #pragma unroll
@@ -481,6 +500,7 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
       __builtin_amdgcn_sched_group_barrier(0x402, 3, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
+    copy(2);
     sf_lds_reads_done(kf);
     read_v<decltype(OV)::value>(va, vf);
     __builtin_amdgcn_sched_barrier(0);
@@ -501,6 +521,7 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
       __builtin_amdgcn_sched_group_barrier(0x402, 6, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
+    copy(3);
     sf_lds_reads_done(vf);
     if (masked) bad = bad || any_not_finite(vf);
   };
@@ -516,8 +537,8 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
     for (int ks = 0; ks < 8; ++ks) ka[ks] = b0 + koff[ks];
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) va[dt] = b0 + voff[dt];
+    aim(k + kAhead);
     sf_wait_vm_barrier<(kAhead - 2) * 4>();
-    issue(k + kAhead);
     step(k, sa, sb, pb, pa, ka, Int<kSlot>{}, va, Int<0>{});
     if (k + 1 == nst) {   // (workgroup-uniform) the last: its P.V follows from the b side
       pb[0] = pa[0];
@@ -527,8 +548,8 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
     const sf_lds_off b1 = sf_lds_addr(ring) + ((k + 2) % kRing) * kSlot;
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) ka[ks] = b1 + koff[ks];
+    aim(k + 1 + kAhead);
     sf_wait_vm_barrier<(kAhead - 2) * 4>();
-    issue(k + 1 + kAhead);
     step(k + 1, sb, sa, pa, pb, ka, Int<0>{}, va, Int<kSlot>{});
   }
   sf_wait_vm_barrier<0>();   // drain the copies past the range's end
@@ -567,7 +588,7 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
                      float* __restrict__ ws_ml) {
   __shared__ __attribute__((aligned(16))) uint8_t ring[4 * kSlot];
   __shared__ int s_bad[4];
-  const Item it = find_item(c);
+  const Item it = find_item<true>(c);
   const Seq& s = c.s[it.si];
   const int lane = threadIdx.x & 63, hf = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // wave-uniform
@@ -843,7 +864,7 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
                       float scale_log2, float decay, float* __restrict__ ws) {
   // K rows of the four waves (16 KB each), slot 0, the stages' lse (256 bytes a slot)
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * 2 * kHalf + kQSlot + kMassRing * 256];
-  const Item it = find_item(c);
+  const Item it = find_item<false>(c);
   const Seq& s = c.s[it.si];
   const MassSeq& ms = c.mass[it.si];
   const int tile = s.tiles - 1 - it.tile;   // the first keys (the most rows) first
@@ -858,18 +879,22 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
   const int nst = max(0, min(c.spr, all - i0));
   const int qb = rows.m0 * G + 32 * i0, q_end = rows.m1 * G;
   const int kw0 = k0 + 64 * wv;   // the wave's first key
-  // row_end by a multiplication
-  auto end_of = [&](int m) { return P - n + min(n, (c.div_block.of(m) + 1) * (int)c.div_block.d); };
-  auto q_at = [&](int qi) {
-    const int m = c.div_g.of(qi);
-    return (size_t)(s.row0 + m) * c.H + it.h * G + (qi - m * G);
+  // this lane's query qi as a byte offset into its sequence's rows of q (of lse: / 64)
+  const uint32_t row_gap = (uint32_t)(c.H - G) * kRowBytes;
+  auto q_off = [&](int qi) {
+    return (uint32_t)qi * kRowBytes + (uint32_t)c.div_g.of(qi) * row_gap;
   };
+  const char* const qh = reinterpret_cast<const char*>(q + ((size_t)s.row0 * c.H + it.h * G) * kHD);
+  const char* const lseh = reinterpret_cast<const char*>(lse + (size_t)s.row0 * c.H + it.h * G);
 
   uint8_t* const kmine = lds + wv * 2 * kHalf;
   uint8_t* const lse_at = lds + 4 * 2 * kHalf + kQSlot;
   auto slot = [&](int i) {
     return i % kMassRing == 0 ? lds + 4 * 2 * kHalf : lds + (i % kMassRing - 1) * kQSlot;
   };
+  uint32_t unit[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) unit[u] = (uint32_t)copy_unit(lane, 8 * wv + 4 * u, false) * 2;
   // stage i's queries (wave w: 8 rows) and their lse: past the range its last stage again,
   // past the queries the last query
   auto issue = [&](int i) {
@@ -877,12 +902,11 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int r0 = 8 * wv + 4 * u;
-      sf_lds_dma16(q + q_at(min(q0 + r0 + (lane >> 4), q_end - 1)) * kHD +
-                       copy_unit(lane, r0, false),
+      sf_lds_dma16(qh + (q_off(min(q0 + r0 + (lane >> 4), q_end - 1)) + unit[u]),
                    slot(i) + r0 * kRowBytes);
     }
-    // (every wave its own copy of the lse would cost LDS: all write the same values)
-    lds_dma4(lse + q_at(min(q0 + (lane & 31), q_end - 1)), lse_at + 256 * (i % kMassRing));
+    // (all four waves write the same values: the copies a wave counts stay alike)
+    lds_dma4(lseh + q_off(min(q0 + (lane & 31), q_end - 1)) / 64, lse_at + 256 * (i % kMassRing));
   };
 
   float acc[2][16], total = 0.f;
@@ -947,18 +971,28 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
     for (int i = 1; i < kMassRing - 1; ++i) issue(i);
 
     const sf_lds_off lse_addr = sf_lds_addr(lse_at) + 4 * lane;
-    // S^T of a stage (both key tiles) and its queries' -lse in base 2
-    auto scores = [&](int i, sf_f32x16 (&out)[2], float& nl) {
+    // Stages [skip0, skip1) hold a query that sees one of the wave's keys, and in [full0,
+    // full1) every query sees all of them: rows from the first that sees the last key to
+    // the last whose window reaches the first.
+    const int kw1 = min(kw0 + 64, P) - 1;   // (a wave behind the last key: none)
+    const Rows some = seen_rows(kw0, kw1, n, P, c.block, c.window, c.sinks);
+    const int full_m0 = seen_rows(kw1, kw1, n, P, c.block, 0, 0).m0;
+    const int full_m1 = kw1 < c.sinks ? n : seen_rows(kw0, kw0, n, P, c.block, c.window, 0).m1;
+    const bool none = kw0 >= P || some.m1 <= some.m0;
+    const int skip0 = none ? 0 : (some.m0 * G - qb) >> 5;
+    const int skip1 = none ? 0 : (some.m1 * G - qb + 31) >> 5;
+    const int full0 = (full_m0 * G - qb + 31) >> 5, full1 = (min(full_m1 * G, q_end) - qb) >> 5;
+
+    auto read_q = [&](int i, sf_u32x4 (&qf)[8], uint32_t& w) {
       sf_lds_off ka[8];
       const sf_lds_off b = sf_lds_addr(slot(i));
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) ka[ks] = b + koff[ks];
-      sf_u32x4 qf[8];
       read_k<0>(ka, qf);
-      uint32_t w = lds_read4(lse_addr + 256 * (i % kMassRing));
-      sf_lds_reads_done(qf);
-      sf_pin(w);
-      nl = -kLog2e * __uint_as_float(w);
+      w = lds_read4(lse_addr + 256 * (i % kMassRing));
+    };
+    // S^T of a stage (both key tiles)
+    auto scores = [&](const sf_u32x4 (&qf)[8], sf_f32x16 (&out)[2]) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -969,27 +1003,45 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
         for (int t = 0; t < 2; ++t)
           out[t] = mfma32(sf_as_bf16x8(kf[t][ks]), sf_as_bf16x8(qf[ks]), out[t]);
     };
+    // stage i: its scores in sc, its queries' -lse (base 2) in nl; stage i + 1's to sn, nn
     auto step = [&](int i, sf_f32x16 (&sc)[2], const float& nl, sf_f32x16 (&sn)[2], float& nn) {
       // stage i + 1 has landed, and every wave is through with stage i - 1's slot
       sf_wait_vm_barrier<(kMassRing - 3) * 3>();
       issue(i + kMassRing - 1);
-      scores(i + 1, sn, nn);
-      const int q0 = qb + 32 * i;
-      const int m_first = c.div_g.of(q0), m_last = c.div_g.of(min(q0 + 31, q_end - 1));
-      const bool skip = end_of(m_last) <= kw0 ||
-                        (kw0 >= c.sinks && row_lo(m_first, n, P, c.window) > kw0 + 63);
-      const bool full = q0 + 31 < q_end && end_of(m_first) >= min(kw0 + 64, P) &&
-                        (kw0 + 63 < c.sinks || row_lo(m_last, n, P, c.window) <= kw0);
-      if (full) {
+      sf_u32x4 qf[8];
+      uint32_t w;
+      read_q(i + 1, qf, w);
+      __builtin_amdgcn_sched_barrier(0);
+      auto weights = [&](int t) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          sc[t][j] = __builtin_amdgcn_exp2f(fmaf(sc[t][j], scale_log2, nl));
+      };
+      weights(0);
+      sf_pin(sc[0]);   // (here, not at its use)
+      __builtin_amdgcn_sched_barrier(0);
+      sf_lds_reads_done(qf);
+      sf_pin(w);
+      nn = -kLog2e * __uint_as_float(w);
+      scores(qf, sn);
+      weights(1);
+      sf_pin(sc[1]);
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, 2, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (i >= full0 && i < full1) {   // wave-uniform
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            acc[t][j] += __builtin_amdgcn_exp2f(fmaf(sc[t][j], scale_log2, nl));
-      } else if (!skip) {
-        const int qi = q0 + (lane & 31);
+          for (int j = 0; j < 16; ++j) acc[t][j] += sc[t][j];
+      } else if (i >= skip0 && i < skip1) {
+        const int qi = qb + 32 * i + (lane & 31);
         const int m = c.div_g.of(min(qi, q_end - 1));
-        const int end = qi < q_end ? end_of(m) : 0;
+        const int end =
+            qi < q_end ? P - n + min(n, (c.div_block.of(m) + 1) * (int)c.div_block.d) : 0;
         const int lo = qi < q_end ? row_lo(m, n, P, c.window) : 0;
         const int sinks = qi < q_end ? c.sinks : 0;
 #pragma unroll
@@ -997,14 +1049,21 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const int key = kw0 + 32 * t + 8 * (j >> 2) + 4 * hf + (j & 3);
-            const float p = __builtin_amdgcn_exp2f(fmaf(sc[t][j], scale_log2, nl));
-            acc[t][j] += seen_key(key, end, lo, sinks) ? p : 0.f;
+            acc[t][j] += seen_key(key, end, lo, sinks) ? sc[t][j] : 0.f;
           }
       }
     };
     sf_f32x16 sa[2], sb[2];
     float na, nb;
-    scores(0, sa, na);
+    {
+      sf_u32x4 qf[8];
+      uint32_t w;
+      read_q(0, qf, w);
+      sf_lds_reads_done(qf);
+      sf_pin(w);
+      na = -kLog2e * __uint_as_float(w);
+      scores(qf, sa);
+    }
 #pragma unroll 1
     for (int i = 0; i < nst; i += 2) {
       step(i, sa, na, sb, nb);
@@ -1051,7 +1110,8 @@ bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 int make_call(const sf_kv_seq* seqs, int n_seqs, int page_size, int block, int window, int sinks,
               int H, int Hkv, int hd, float scaling, bool mass, Call& c) {
   if (!seqs) return SF_ERR_ARG;
-  if (hd != kHD || H < 1 || Hkv < 1 || H % Hkv != 0 || H / Hkv > kMaxG) return SF_ERR_SHAPE;
+  if (hd != kHD || H < 1 || Hkv < 1 || H % Hkv != 0 || H / Hkv > kMaxG || H > kMaxH)
+    return SF_ERR_SHAPE;
   if (n_seqs < 1 || n_seqs > kMaxSeqs) return SF_ERR_SHAPE;
   if (block < 1 || window < 0 || sinks < 0) return SF_ERR_SHAPE;
   // (the running maximum is the scores' before scaling)

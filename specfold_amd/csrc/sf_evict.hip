@@ -5,10 +5,13 @@
 // k = keep - sinks - recent others with the largest mass, equal ones by the lower index.
 //  * select: one workgroup per (layer, kv head).  The masses are mapped to unsigned
 //    integers of the same order and stay in registers; the k-th largest value is built
-//    two bits at a time from the top by counting the keys that are not below each
-//    candidate (ballots; exact, no atomics), until the count is k or no bit is left; two
-//    ballot scans number the ties and the kept keys in index order.  Bound by the steps'
-//    barriers (about 0.5 us each).
+//    eight bits at a time from the top: a histogram in LDS of the digit of the keys that
+//    agree so far (integer counts, whatever their order; one copy: four, a lane in its
+//    own, gained nothing), which every wave sums from the top for itself, so a step has
+//    one barrier.  It ends as soon as just the keys that are needed are left.  Two ballot
+//    scans number the ties and the kept keys in index order.  (Two bits a step by counting
+//    with ballots, no histogram: 56 lists of 1056 keys with their copy 33 us, 25 so; 320
+//    of 16384 542 and 524.)
 //  * move: the kept rows to slots 0 .. keep - 1, ascending, bound by reading and writing
 //    them once.  Into another cache every 128 rows are a workgroup's.  In place slot j
 //    takes a row from a slot >= j, so a workgroup goes up the slots of its (layer, kv
@@ -22,6 +25,7 @@ constexpr int kHD = 128;
 constexpr int kMaxKeys = 32768;
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
+constexpr int kSteps = 4;    // of 8 bits
 
 // The order of a float as an unsigned integer: NaN above all, -0 as 0.
 SF_DEV uint32_t order_of(float x) {
@@ -35,8 +39,7 @@ __global__ __launch_bounds__(kSelThreads) void sf_evict_select_kernel(
     const float* mass, long long mass_layer, long long mass_head, int Hkv, int P, int sinks,
     int recent, int keep, int32_t* __restrict__ kept, float* mass_out, long long out_layer,
     long long out_head, int zero_to) {
-  __shared__ int s_red[2][64];
-  __shared__ int s_above[kSelWaves];
+  __shared__ sf_u32x4 s_hist[kSteps * 64];
   __shared__ int s_cnt[PER * kSelWaves];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int l = blockIdx.x / Hkv, h = blockIdx.x - l * Hkv;
@@ -52,33 +55,47 @@ __global__ __launch_bounds__(kSelThreads) void sf_evict_select_kernel(
   const int need = keep - sinks - recent;   // <= last - sinks
   // thr: the need-th largest, or (exact) a bound that just the `need` largest reach
   uint32_t thr = 0;
+  int ties = need;   // of the keys that agree with thr in the digits found: how many stay
   bool exact = false;
   if (need > 0) {
+    for (int i = tid; i < kSteps * 64; i += kSelThreads)
+      s_hist[i] = sf_u32x4{0u, 0u, 0u, 0u};
+    __syncthreads();
 #pragma unroll 1
-    for (int sh = 30; sh >= 0 && !exact; sh -= 2) {   // workgroup-uniform
-      int n[3];
+    for (int sh = 24; sh >= 0 && !exact; sh -= 8) {   // workgroup-uniform
+      int* hist = reinterpret_cast<int*>(s_hist) + (sh >> 3) * 256;
 #pragma unroll
-      for (int d = 0; d < 3; ++d) {
-        const uint32_t cand = thr | ((uint32_t)(d + 1) << sh);
-        n[d] = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) n[d] += __popcll(__ballot(key[i] >= cand));
-      }
-      int* red = s_red[(sh >> 1) & 1];   // (two in turn: one barrier a step)
-      if (lane < 3) red[wv * 4 + lane] = lane == 0 ? n[0] : lane == 1 ? n[1] : n[2];
+      for (int i = 0; i < PER; ++i)
+        if (key[i] != 0u && ((key[i] ^ thr) >> sh) < 256u)
+          atomicAdd(&hist[key[i] >> sh & 255u], 1);
       __syncthreads();
-      // lane 4w + d: wave w's count of candidate d + 1; then the sums over the waves
-      int t = (lane & 3) < 3 ? red[lane] : 0;
+      // every wave: lane x has the digits 4x .. 4x + 3, at[d] counts them and those above
+      const sf_u32x4 w = reinterpret_cast<const sf_u32x4*>(hist)[lane];
+      int n[4], at[4], sum = 0;
 #pragma unroll
-      for (int o = 4; o <= 32; o <<= 1) t += __shfl_xor(t, o, 64);
-      const int digit = __popcll(__ballot(t >= need && (lane & 3) < 3) & 7ull);   // falling counts
-      if (digit > 0) {
-        thr |= (uint32_t)digit << sh;
-        exact = __shfl(t, digit - 1, 64) == need;
+      for (int d = 3; d >= 0; --d) {
+        n[d] = (int)w[d];
+        sum += n[d];
+        at[d] = sum;
       }
+      int up = sum;
+#pragma unroll
+      for (int o = 1; o <= 32; o <<= 1) {
+        const int t = __shfl(up, lane + o < 64 ? lane + o : lane, 64);
+        up += lane + o < 64 ? t : 0;
+      }
+      up -= sum;
+      // the digit: the largest with `ties` keys at or above it
+      int mine = -1, over = 0, in_it = 0;
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        if (at[d] + up >= ties) mine = d, over = at[d] + up - n[d], in_it = n[d];
+      const int top = __popcll(__ballot(mine >= 0)) - 1;   // (lanes 0 .. top)
+      thr |= (uint32_t)(4 * top + __shfl(mine, top, 64)) << sh;
+      ties -= __shfl(over, top, 64);
+      exact = __shfl(in_it, top, 64) == ties;
     }
   }
-  int above = 0;
   uint32_t keeps = 0, equal = 0;   // bit i: key i of this thread
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -88,7 +105,6 @@ __global__ __launch_bounds__(kSelThreads) void sf_evict_select_kernel(
     const bool over = in_it & (exact ? key[i] >= thr : key[i] > thr);
     if (t < P && (!mid || over)) keeps |= 1u << i;
     if (in_it && !exact && key[i] == thr) equal |= 1u << i;
-    above += over ? 1 : 0;
   }
   // index-order numbering of the flagged keys: s_cnt holds, for each 64 of them, how
   // many are flagged in front
@@ -121,12 +137,8 @@ __global__ __launch_bounds__(kSelThreads) void sf_evict_select_kernel(
     __syncthreads();
   };
   const unsigned long long below = (1ull << lane) - 1;
-  if (need > 0 && !exact) {   // of the equal ones the first need - (those above)
-    for (int o = 32; o >= 1; o >>= 1) above += __shfl_xor(above, o, 64);
-    if (lane == 0) s_above[wv] = above;
+  if (need > 0 && !exact) {   // of the equal ones the first
     scan(equal);
-    int ties = need;
-    for (int w = 0; w < kSelWaves; ++w) ties -= s_above[w];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const unsigned long long b = __ballot(equal >> i & 1u);

@@ -584,16 +584,15 @@ constexpr int kMassKeys = 256;
 constexpr int kMassRanges = 16;   // ranges of queries at most (bounds the workspace)
 SF_IDX int mass_stages(const Rows& r, int G) { return r.m1 > r.m0 ? ((r.m1 - r.m0) * G + 31) / 32 : 0; }
 
-// x / d by a multiplication, for 0 <= x < 2^20 and 1 <= d <= 2^15 with x * d < 2^32
-// (ceil(2^32 / d) is off by less than 1 / 2^32 of x * d from x / d's next step).
+// x / d by a multiplication, for x >= 0 and d >= 1 with x * d < 2^30: 2x / 2d, where
+// mul = ceil(2^32 / 2d) fits also for d = 1, and is off by so little that 2x * mul / 2^32
+// stays below the next multiple of 1 / d.
 struct Div {
   unsigned d, mul;
-  SF_IDX int of(int x) const {
-    return d == 1 ? x : (int)(((unsigned long long)(unsigned)x * mul) >> 32);
-  }
+  SF_IDX int of(int x) const { return (int)(((2ull * (unsigned)x) * mul) >> 32); }
 };
 inline Div make_div(int d) {
-  return Div{(unsigned)d, d == 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d)};
+  return Div{(unsigned)d, (unsigned)(((1ull << 32) + 2 * d - 1) / (2 * d))};
 }
 
 // Ranges a query's keys are cut into at most, by the rows of the call (bounds the

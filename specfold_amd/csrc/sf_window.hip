@@ -298,6 +298,8 @@ SF_DEV void write_partial(const sf_f32x16 (&acc)[4], float m, float l, int hf, f
 // tiles, the last tile of a sequence (the most keys) first, then the range: blocks of
 // ranges that a tile does not have end at once, and stand behind those that work
 // (INNER = false; 1494 causal rows of 12 / 2 heads: 67 us with the ranges inside, 53).
+// Range r starts r tiles on, or with 4 kv heads and 16 tiles the even tiles, which have
+// more ranges, would all be on the same XCDs and be more than these hold at once.
 // INNER: the ranges of a tile side by side, for the few-query kernel (8 tokens over 8
 // sequences of unlike lengths: 31 us, 38 with the ranges outside).
 struct Item {
@@ -309,7 +311,7 @@ SF_DEV Item find_item(const Call& c) {
   it.h = blockIdx.x % c.Hkv;
   const int rest = blockIdx.x / c.Hkv;
   it.r = INNER ? rest % c.nr : rest / c.tiles;
-  const int tt = INNER ? rest / c.nr : rest % c.tiles;
+  const int tt = INNER ? rest / c.nr : (rest - it.r * c.tiles + it.r) % c.tiles;
   it.si = 0;
   while (tt >= c.s[it.si].tile0 + c.s[it.si].tiles) ++it.si;
   it.tile = c.s[it.si].tiles - 1 - (tt - c.s[it.si].tile0);
@@ -837,6 +839,7 @@ struct MassCall : Call {
   MassSeq mass[kMaxSeqs];
   Div div_g, div_block;
   int keys;   // of all sequences
+  int last_first;
 };
 // 4 bytes per lane of a direct copy, and an LDS read of 4 bytes without a wait.
 #if defined(__HIPCC__)
@@ -867,7 +870,9 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
   const Item it = find_item<false>(c);
   const Seq& s = c.s[it.si];
   const MassSeq& ms = c.mass[it.si];
-  const int tile = s.tiles - 1 - it.tile;   // the first keys (the most rows) first
+  // the first keys (the most rows) first; where every tile has as many, the last ones, which
+  // may be few and then make room for another tile early
+  const int tile = c.last_first ? it.tile : s.tiles - 1 - it.tile;
   const int lane = threadIdx.x & 63, hf = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // wave-uniform
   const int G = c.H / c.Hkv, P = s.length, n = s.rows;
@@ -914,6 +919,11 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
+  // the key this lane ends with, and what that had (on its way beside the K rows)
+  const int x = lane & 31;
+  const int key = kw0 + 32 * (x >> 4) + 8 * ((x & 15) >> 2) + 4 * hf + (x & 3);
+  float had = 0.f;
+  if (c.nr == 1 && ms.in && key < P) had = decay * ms.in[it.h * ms.in_stride + key];
   // acc joined over the lanes and added to the total of this lane's key: lane x of a half
   // ends with value x of the 32 (key tile x / 16)
   auto flush = [&]() {
@@ -971,16 +981,13 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
     for (int i = 1; i < kMassRing - 1; ++i) issue(i);
 
     const sf_lds_off lse_addr = sf_lds_addr(lse_at) + 4 * lane;
-    // Stages [skip0, skip1) hold a query that sees one of the wave's keys, and in [full0,
-    // full1) every query sees all of them: rows from the first that sees the last key to
-    // the last whose window reaches the first.
+    // In stages [full0, full1) every query sees all of the wave's keys: rows from the first
+    // that sees the last key to the last whose window reaches the first.
     const int kw1 = min(kw0 + 64, P) - 1;   // (a wave behind the last key: none)
     const Rows some = seen_rows(kw0, kw1, n, P, c.block, c.window, c.sinks);
     const int full_m0 = seen_rows(kw1, kw1, n, P, c.block, 0, 0).m0;
     const int full_m1 = kw1 < c.sinks ? n : seen_rows(kw0, kw0, n, P, c.block, c.window, 0).m1;
     const bool none = kw0 >= P || some.m1 <= some.m0;
-    const int skip0 = none ? 0 : (some.m0 * G - qb) >> 5;
-    const int skip1 = none ? 0 : (some.m1 * G - qb + 31) >> 5;
     const int full0 = (full_m0 * G - qb + 31) >> 5, full1 = (min(full_m1 * G, q_end) - qb) >> 5;
 
     auto read_q = [&](int i, sf_u32x4 (&qf)[8], uint32_t& w) {
@@ -1032,26 +1039,27 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
         __builtin_amdgcn_sched_group_barrier(0x402, 2, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
-      if (i >= full0 && i < full1) {   // wave-uniform
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) acc[t][j] += sc[t][j];
-      } else if (i >= skip0 && i < skip1) {
+      if (i < full0 || i >= full1) {   // wave-uniform
         const int qi = qb + 32 * i + (lane & 31);
         const int m = c.div_g.of(min(qi, q_end - 1));
-        const int end =
-            qi < q_end ? P - n + min(n, (c.div_block.of(m) + 1) * (int)c.div_block.d) : 0;
-        const int lo = qi < q_end ? row_lo(m, n, P, c.window) : 0;
-        const int sinks = qi < q_end ? c.sinks : 0;
+        const bool any = qi < q_end && !none;
+        const int end = any ? P - n + min(n, (c.div_block.of(m) + 1) * (int)c.div_block.d) : 0;
+        const int lo = any ? row_lo(m, n, P, c.window) : 0;
+        const int sinks = any ? c.sinks : 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const int key = kw0 + 32 * t + 8 * (j >> 2) + 4 * hf + (j & 3);
-            acc[t][j] += seen_key(key, end, lo, sinks) ? sc[t][j] : 0.f;
+            sc[t][j] = seen_key(key, end, lo, sinks) ? sc[t][j] : 0.f;
           }
+        sf_pin(sc[0]);
+        sf_pin(sc[1]);
       }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[t][j] += sc[t][j];
     };
     sf_f32x16 sa[2], sb[2];
     float na, nb;
@@ -1074,11 +1082,8 @@ sf_window_mass_kernel(const uint16_t* __restrict__ q, const float* __restrict__ 
   }
 
   flush();
-  const int x = lane & 31;
-  const int key = kw0 + 32 * (x >> 4) + 8 * ((x & 15) >> 2) + 4 * hf + (x & 3);
   if (key >= P) return;
   if (c.nr == 1) {
-    const float had = ms.in ? decay * ms.in[it.h * ms.in_stride + key] : 0.f;
     ms.out[it.h * ms.out_stride + key] = had + total;
   } else {
     sf_handoff_store(ws + ((size_t)it.r * c.Hkv + it.h) * c.keys + ms.key0 + key, total);
@@ -1098,10 +1103,17 @@ __global__ __launch_bounds__(kMassKeys) void sf_window_mass_merge_kernel(
   const Rows rows = seen_rows(k0, min(k0 + kMassKeys, s.length) - 1, s.rows, s.length, c.block,
                               c.window, c.sinks);
   const int nm = (mass_stages(rows, c.H / c.Hkv) + c.spr - 1) / c.spr;
-  float sum = 0.f;
-  for (int r = 0; r < nm; ++r)
-    sum += sf_handoff_load(ws + ((size_t)r * c.Hkv + h) * c.keys + ms.key0 + key);
   const float had = ms.in ? decay * ms.in[h * ms.in_stride + key] : 0.f;
+  float sum = 0.f;
+  for (int r0 = 0; r0 < nm; r0 += 8) {   // (8 loads on their way together)
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      v[u] = sf_handoff_load(ws + ((size_t)min(r0 + u, nm - 1) * c.Hkv + h) * c.keys + ms.key0 +
+                             key);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) sum += r0 + u < nm ? v[u] : 0.f;
+  }
   ms.out[h * ms.out_stride + key] = had + sum;
 }
 
@@ -1166,7 +1178,8 @@ void plan_spread(Call& c, long long work, int longest, int cap, int slots, Cost 
     const double items = c.Hkv * (nr == 1 ? (double)c.tiles : (double)work / spr + 0.5 * c.tiles);
     const double one = spr + (nr == 1 ? fix.one : fix.many + fix.many * (nr / 16) / 4);
     const double all = (c.Hkv * (double)work + items * (one - spr)) / slots;
-    const double cost = items <= slots ? one : all + 0.5 * one;
+    // (an XCD may get a few more than its share: one item too many doubles the time)
+    const double cost = items <= slots - slots / 32 ? one : all + 0.5 * one;
     if (nr == 1 || cost < best) {
       best = cost;
       c.nr = (longest + spr - 1) / spr;
@@ -1298,6 +1311,7 @@ extern "C" int sf_attn_key_mass(const uint16_t* q, const float* lse, const sf_kv
   if (c.keys == 0) return SF_OK;
   if (!workspace || !aligned(workspace)) return SF_ERR_ARG;
   if (workspace_bytes < sf_attn_key_mass_workspace_bytes(c.keys, Hkv)) return SF_ERR_WORKSPACE;
+  c.last_first = work == (long long)longest * c.tiles;
   plan_spread(c, work, longest, kMassRanges, 2 * kCUs, Cost{6, 10}, 1);
   hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
   float* ws = reinterpret_cast<float*>(workspace);

@@ -517,11 +517,13 @@ typedef struct sf_kv_seq {
  * them.  Results do not depend on the order of pages or of workgroups.
  * workspace: sf_attn_window_workspace_bytes(rows, H) bytes, 16-byte aligned; calls that
  * share one must not overlap (two captured graphs that may replay at once need two).
- * Limits: hd == 128, H % Hkv == 0, H/Hkv <= 16, H <= 256, 1 <= n_seqs <= 32, 0 <= rows <= length
- * <= 32768 (each sequence), block >= 1, window >= 0, sinks >= 0, scaling positive and
- * finite; page_size 16, 32, 64 or
- * 128 where a page_table is given; strides multiples of 8 elements, 16-byte aligned
- * pointers.
+ * Lengths and rows are the host's at the call: a captured call replays with them, reading
+ * the pages and the page table as they then are.  o, lse and the workspace overlap none of
+ * what is read.
+ * Limits: hd == 128, H % Hkv == 0, H/Hkv <= 16, H <= 256, 1 <= n_seqs <= 32, 0 <= rows <=
+ * length <= 32768 (each sequence), block >= 1, window >= 0, sinks >= 0, scaling positive
+ * and finite; page_size 16, 32, 64 or 128 where a page_table is given; strides multiples
+ * of 8 elements, 16-byte aligned pointers.
  */
 size_t sf_attn_window_workspace_bytes(int rows, int H);
 int sf_attn_window(const uint16_t* q, const sf_kv_seq* seqs, int n_seqs, int page_size, int block,
@@ -533,7 +535,9 @@ int sf_attn_window(const uint16_t* q, const sf_kv_seq* seqs, int n_seqs, int pag
  *   mass_out[h][t] = decay * mass_in[h][t] + sum over the rows that see t and the H/Hkv
  *                    q-heads of kv head h of exp(scaling * q . k - lse),   t < length
  * with lse as sf_attn_window wrote it; entries at and behind length are not touched.
- * fp32 sums in a fixed order (no atomics).  Masks and limits as sf_attn_window;
+ * fp32 sums in a fixed order (no atomics).  A mass_out overlaps no other sequence's
+ * mass_in or mass_out, nor its own mass_in but as the very same array.  A row whose lse is
+ * NaN or -inf reaches the keys it sees only.  Masks and limits as sf_attn_window;
  * 0 <= decay <= 1.  workspace: sf_attn_key_mass_workspace_bytes(keys, Hkv) bytes, keys =
  * the sum of the sequences' lengths, 16-byte aligned.
  */
@@ -552,7 +556,7 @@ int sf_attn_key_mass(const uint16_t* q, const float* lse, const sf_kv_seq* seqs,
  *   kept[l][h][j]  int32, the old slot of slot j
  *   mass_out       the kept keys' mass, [l][h] rows at mass_out_layer / _head strides;
  *                  may be NULL; where it is `mass` itself (same strides), entries
- *                  keep .. P - 1 are set to 0
+ *                  keep .. P - 1 are set to 0; else it overlaps nothing of it
  * Keys keep the RoPE angles they were appended with.  Limits: hd == 128, 1 <= P <= 32768,
  * sinks + recent <= keep <= P, keep >= 1; page sizes and alignment as sf_attn_window, a
  * page_table in both; an id outside [0, pages) is read as page 0 and not written.

@@ -277,6 +277,14 @@ extern "C" int sf_kv_evict(const float* mass, long long mass_layer, long long ma
   if (st != SF_OK) return st;
   if (mass_out == mass && (mass_out_layer != mass_layer || mass_out_head != mass_head))
     return SF_ERR_ARG;
+  if (mass_out) {   // its rows must not overlap
+    const long long n = mass_out == mass ? P : keep;
+    const bool heads_inside = Hkv == 1 || layers == 1 || mass_out_head <= mass_out_layer;
+    const long long head_span = Hkv > 1 ? mass_out_head * (Hkv - 1) : 0;
+    const long long layer_span = layers > 1 ? mass_out_layer * (layers - 1) : 0;
+    if (Hkv > 1 && mass_out_head < n + (heads_inside ? 0 : layer_span)) return SF_ERR_SHAPE;
+    if (layers > 1 && mass_out_layer < n + (heads_inside ? head_span : 0)) return SF_ERR_SHAPE;
+  }
   // the same pool through the same table: the same mapping, in place
   const bool in_place = from->k == to->k && from->page_table == to->page_table;
   if (in_place && (from->v != to->v || from->layer_stride != to->layer_stride ||

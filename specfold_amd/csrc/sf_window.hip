@@ -1156,6 +1156,12 @@ int make_call(const sf_kv_seq* seqs, int n_seqs, int page_size, int block, int w
         if (Hkv > 1 && (x.mass_out_stride < x.length || (x.mass_in && x.mass_in_stride < x.length)))
           return SF_ERR_SHAPE;
         if (x.mass_in == x.mass_out && x.mass_in_stride != x.mass_out_stride) return SF_ERR_ARG;
+        // sequences that share what one of them writes
+        for (int j = 0; j < i; ++j)
+          if (x.length > 0 && seqs[j].length > 0 &&
+              (x.mass_out == seqs[j].mass_out || x.mass_out == seqs[j].mass_in ||
+               x.mass_in == seqs[j].mass_out))
+            return SF_ERR_ARG;
       }
     }
     c.s[i] = Seq{x.k, x.v, x.page_table, x.page_stride, x.head_stride, x.length, x.rows, c.rows,

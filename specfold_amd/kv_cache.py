@@ -196,15 +196,25 @@ class PagedBatch:
         for c, n in zip(self.caches, self.rows):
             if not isinstance(c, (PagedKVCache, ContiguousMirror)):
                 raise TypeError("a batch takes PagedKVCache or ContiguousMirror caches")
-            if c.Hkv != self.Hkv or c.length_dev.device != self.device or \
+            if (c.Hkv, c.hd) != (self.Hkv, self.hd) or c.length_dev.device != self.device or \
                     (isinstance(c, PagedKVCache) and c.page_size != self.page_size):
-                raise ValueError("the caches of a batch share kv heads, page size and device")
+                raise ValueError("the caches of a batch share kv heads, head size, page size and "
+                                 "device")
             if n < 0:
                 raise ValueError("a row count must not be negative")
         self._layers: Dict[int, object] = {}
+        self._buffers: list = [None] * len(self.caches)   # as the arrays point to them
 
     def seqs(self, li: int):
         """Layer li's sf_kv_seq array at the caches' present lengths."""
+        held = self._buffers
+        for i, c in enumerate(self.caches):
+            k, v, table = (c.k_pages, c.v_pages, c.page_table) if isinstance(c, PagedKVCache) \
+                else (c.k, c.v, None)
+            h = held[i]
+            if h is None or h[0] is not k or h[1] is not v or h[2] is not table:
+                self._layers.clear()    # (a cache given other buffers)
+                held[i] = k, v, table
         arr, views, lengths = self._layers.get(li, (None, [], None))
         if arr is None:
             arr = (_lib.KVSeq * len(self.caches))()

@@ -112,6 +112,8 @@ MASS = [
     ([(999, 3000), (70, 170)], 28, 4, 1, 0, 0, 16),
     ([(1025, 2049)], 40, 8, 32, 333, 17, 128),
     ([(600, 1800)], 16, 1, 16, 200, 130, 16),
+    # (ranges of more stages than are summed lane by lane)
+    ([(2500, 2600)], 28, 4, 32, 0, 0, 16),
 ]
 
 

@@ -293,7 +293,13 @@ def _evict(lib, **over):
     (dict(page_size=24), SHAPE), (dict(to_page_size=8), SHAPE), (dict(pages=3), SHAPE),
     (dict(to_pages=1), SHAPE), (dict(page_stride=4), SHAPE), (dict(to_layer_stride=7), SHAPE),
     (dict(to_v=4096 * 5), ARG), (dict(to_head_stride=4096), ARG), (dict(to_page_size=32), ARG),
-    (dict(mass_out=4096, oml=128, omh=63), ARG)])
+    (dict(mass_out=4096, oml=128, omh=63), ARG),
+    # rows of mass_out over each other
+    (dict(mass_out=16384, oml=64, omh=31), SHAPE), (dict(mass_out=4096, mh=63, omh=63, oml=128), SHAPE),
+    (dict(mass_out=16384, layers=3, oml=63, omh=32), SHAPE),
+    (dict(mass_out=16384, layers=3, oml=32, omh=95), SHAPE),
+    (dict(mass_out=16384, layers=3, oml=31, omh=96), SHAPE),
+    (dict(mass_out=16384, layers=3, Hkv=1, oml=0), SHAPE)])
 def test_evict_refusals(over, code):
     assert _evict(_lib.load(), **over) == code
 
@@ -372,6 +378,56 @@ def test_scaling_refused(sim, what, scaling):
             sim.attn_window(q, batch, 0, 4, scaling, torch.empty(3, 512, dtype=BF), ws)
         else:
             sim.attn_key_mass(q, torch.zeros(3, 4), batch, 0, 4, scaling, [torch.zeros(2, 20)], ws)
+
+
+def test_too_many_heads_refused():
+    for what in ("window", "mass"):
+        assert _call(_lib.load(), what, H=272, Hkv=17, mass_out_stride=64) == SHAPE
+
+
+def test_shared_mass_refused(sim):
+    """Two sequences that write one array, or of which one reads what the other writes."""
+    q, ks, vs, caches = make_seqs([(1, 20), (2, 24)], 4, 2, 1, "cpu")
+    batch, lse = PagedBatch(caches, [1, 2]), torch.zeros(3, 4)
+    ws = torch.empty(sim.attn_key_mass_workspace_bytes(44, 2), dtype=torch.uint8)
+    a, b, c = (torch.zeros(2, 24) for _ in range(3))
+    for out, had in (([a, a], None), ([a, b], [b, c]), ([a, b], [c, a])):
+        with pytest.raises(_lib.SpecFoldKernelError):
+            sim.attn_key_mass(q, lse, batch, 0, 4, 0.1, out, ws, mass_in=had)
+    sim.attn_key_mass(q, lse, batch, 0, 4, 0.1, [a, b], ws, mass_in=[c, c])   # reading one is fine
+
+
+def test_batch_follows_its_caches(sim):
+    """A batch that was used before a cache got other buffers (and lengths) reads those; one
+    cache twice in a batch is two sequences."""
+    q, ks, vs, caches = make_seqs([(2, 40)], 4, 2, 1, "cpu")
+    batch, ws = PagedBatch(caches, [2]), torch.empty(1 << 23, dtype=torch.uint8)
+    outs = [torch.empty(2, 512, dtype=BF) for _ in range(3)]
+    sim.attn_window(q, batch, 0, 4, HD ** -0.5, outs[0], ws)
+    caches[0].v_pages.neg_()
+    sim.attn_window(q, batch, 0, 4, HD ** -0.5, outs[1], ws)
+    assert torch.equal(outs[1], -outs[0])
+    caches[0].v_pages = -caches[0].v_pages
+    sim.attn_window(q, batch, 0, 4, HD ** -0.5, outs[2], ws)
+    assert torch.equal(outs[2], outs[0])
+    twice = torch.empty(4, 512, dtype=BF)
+    sim.attn_window(torch.cat([q, q]), PagedBatch(caches * 2, [2, 2]), 0, 4, HD ** -0.5, twice, ws)
+    assert torch.equal(twice, torch.cat([outs[0], outs[0]]))
+    with pytest.raises(ValueError):
+        PagedBatch([caches[0], PagedKVCache(1, 2, 64, 64, page_size=16, device="cpu")], [1, 1])
+
+
+def test_mass_of_a_row_without_a_number(sim):
+    """A row whose lse is NaN or -inf reaches the keys it sees, and no other."""
+    q, ks, vs, caches = make_seqs([(40, 100)], 4, 2, 1, "cpu")
+    ws = torch.empty(sim.attn_key_mass_workspace_bytes(100, 2), dtype=torch.uint8)
+    lse = torch.zeros(40, 4)
+    lse[7] = float("nan")
+    lse[9, 0] = -math.inf
+    out = [torch.zeros(2, 100)]
+    sim.attn_key_mass(q, lse, PagedBatch(caches, [40]), 0, 4, HD ** -0.5, out, ws)
+    assert out[0][:, :68].isnan().all() and out[0][1, 68:].isfinite().all()
+    assert (out[0][0, 68:70] == math.inf).all() and out[0][0, 70:].isfinite().all()
 
 
 def test_extreme_masks(sim):

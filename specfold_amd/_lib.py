@@ -527,9 +527,9 @@ def attn_key_mass(q, lse, batch, li, H, scaling, mass, workspace, mass_in=None, 
     dev, Hkv = q.device, batch.Hkv
     for i, s in enumerate(seqs):
         t, u = mass[i], None if mass_in is None else mass_in[i]
-        stride, n = t.stride(), s.length
-        if t.dtype is not torch.float32 or t.dim() != 2 or t.shape[0] != Hkv or \
-                t.shape[1] < n or stride[1] != 1 or t.device != dev:
+        shape, stride, n = t.shape, t.stride(), s.length
+        if t.dtype is not torch.float32 or len(shape) != 2 or shape[0] != Hkv or \
+                shape[1] < n or stride[1] != 1 or t.device != dev:
             raise _bad_mass("mass", t, Hkv, n, dev)
         s.mass_out, s.mass_out_stride = t.data_ptr(), stride[0]
         if u is t:
@@ -537,9 +537,9 @@ def attn_key_mass(q, lse, batch, li, H, scaling, mass, workspace, mass_in=None, 
         elif u is None:
             s.mass_in = None
         else:
-            stride = u.stride()
-            if u.dtype is not torch.float32 or u.dim() != 2 or u.shape[0] != Hkv or \
-                    u.shape[1] < n or stride[1] != 1 or u.device != dev:
+            shape, stride = u.shape, u.stride()
+            if u.dtype is not torch.float32 or len(shape) != 2 or shape[0] != Hkv or \
+                    shape[1] < n or stride[1] != 1 or u.device != dev:
                 raise _bad_mass("mass_in", u, Hkv, n, dev)
             s.mass_in, s.mass_in_stride = u.data_ptr(), stride[0]
     st = _on_device(load().sf_attn_key_mass, q,
@@ -567,25 +567,27 @@ def kv_evict(mass, length: int, keep: int, sinks: int, recent: int, src, dst, ke
     for nm, t, n in (("mass", mass, length), ("mass_out", mass_out, keep)):
         if t is None and nm == "mass_out":
             continue
-        if t.dtype != torch.float32 or t.dim() != 3 or tuple(t.shape[:2]) != (L, Hkv) or \
-                t.shape[2] < n or t.stride(2) != 1:
+        shape = t.shape
+        if t.dtype is not torch.float32 or len(shape) != 3 or shape[0] != L or \
+                shape[1] != Hkv or shape[2] < n or t.stride(2) != 1:
             raise ValueError(f"{nm}: expected float32 [{L}, {Hkv}, >= {n}] with contiguous rows, "
                              f"got {t.dtype} {tuple(t.shape)}")
     pages = []
     for c in (src, dst):
         _need(c.k_pages, "k_pages", torch.bfloat16)
         _need(c.v_pages, "v_pages", torch.bfloat16)
+        layer, page, head = c.k_pages.stride()[:3]
         pages.append(KVPages(c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.page_table.data_ptr(),
-                             c.k_pages.stride(0), c.k_pages.stride(1), c.k_pages.stride(2),
-                             c.page_size, c.num_pages))
+                             layer, page, head, c.page_size, c.num_pages))
     none = mass_out is None
+    layer, head, _ = mass.stride()
+    out_layer, out_head, _ = (0, 0, 0) if none else mass_out.stride()
     st = _on_device(load().sf_kv_evict, mass,
                     (("kept", kept), ("mass_out", mass_out), ("src", src.k_pages),
                      ("dst", dst.k_pages)), stream,
-                    mass.data_ptr(), mass.stride(0), mass.stride(1), L, Hkv, hd, length, sinks,
-                    recent, keep, ctypes.byref(pages[0]), ctypes.byref(pages[1]), kept.data_ptr(),
-                    None if none else mass_out.data_ptr(), 0 if none else mass_out.stride(0),
-                    0 if none else mass_out.stride(1))
+                    mass.data_ptr(), layer, head, L, Hkv, hd, length, sinks, recent, keep,
+                    ctypes.byref(pages[0]), ctypes.byref(pages[1]), kept.data_ptr(),
+                    None if none else mass_out.data_ptr(), out_layer, out_head)
     _check(st, "sf_kv_evict")
 
 

@@ -203,18 +203,23 @@ class PagedBatch:
             if n < 0:
                 raise ValueError("a row count must not be negative")
         self._layers: Dict[int, object] = {}
-        self._buffers: list = [None] * len(self.caches)   # as the arrays point to them
+        self._kinds = [(c, isinstance(c, PagedKVCache)) for c in self.caches]
+        self._buffers: list = [(None,)] * len(self.caches)   # as the arrays point to them
 
     def seqs(self, li: int):
         """Layer li's sf_kv_seq array at the caches' present lengths."""
         held = self._buffers
-        for i, c in enumerate(self.caches):
-            k, v, table = (c.k_pages, c.v_pages, c.page_table) if isinstance(c, PagedKVCache) \
-                else (c.k, c.v, None)
+        for i, (c, paged) in enumerate(self._kinds):
             h = held[i]
-            if h is None or h[0] is not k or h[1] is not v or h[2] is not table:
-                self._layers.clear()    # (a cache given other buffers)
-                held[i] = k, v, table
+            if paged:
+                if h[0] is c.k_pages and h[1] is c.v_pages and h[2] is c.page_table:
+                    continue
+                held[i] = c.k_pages, c.v_pages, c.page_table
+            else:
+                if h[0] is c.k and h[1] is c.v:
+                    continue
+                held[i] = c.k, c.v
+            self._layers.clear()    # (a cache given other buffers)
         arr, views, lengths = self._layers.get(li, (None, [], None))
         if arr is None:
             arr = (_lib.KVSeq * len(self.caches))()

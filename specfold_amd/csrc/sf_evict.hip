@@ -11,12 +11,14 @@
 //    one barrier.  It ends as soon as just the keys that are needed are left.  Two ballot
 //    scans number the ties and the kept keys in index order.  (Two bits a step by counting
 //    with ballots, no histogram: 56 lists of 1056 keys with their copy 33 us, 25 so; 320
-//    of 16384 542 and 524.)
+//    of 16384 542 and 524.)  Bound by its latencies: 7.5 us for 56 lists of 1056 or 112 of
+//    4095 keys, 41 for 320 of 16384.
 //  * move: the kept rows to slots 0 .. keep - 1, ascending, bound by reading and writing
-//    them once.  Into another cache every 128 rows are a workgroup's.  In place slot j
-//    takes a row from a slot >= j, so a workgroup goes up the slots of its (layer, kv
-//    head) alone: a tile is written when all of its rows have been read, and the rows of
-//    the tile behind it, which no write of this one reaches, are on their way.
+//    them once (2.7 GB at 5.7 TB/s, 115 MB at 5.2).  Into another cache every 128 rows are
+//    a workgroup's.  In place slot j takes a row from a slot >= j, so a workgroup goes up
+//    the slots of its (layer, kv head) alone: a tile is written when all of its rows have
+//    been read, and the rows of the tile behind it, which no write of this one reaches,
+//    are on their way.
 #include "sf_common.h"
 
 namespace {

@@ -327,6 +327,11 @@ SF_DEV Item find_item(const Call& c) {
 // that one's matrix products meet the other's loads; one workgroup of eight waves and 256
 // queries, which copies half as much, measured 506 against 499 us on 8192 rows of 28 / 4
 // heads and 175 against 150 on four shorter runs of rows.
+// Bound by the matrix core and the vector ALU, 40 % of the cycles each and mostly in turn,
+// and by the waits between them: 8192 rows of 28 / 4 heads over themselves 495 us (0.97
+// PFLOP/s; a large library product 1.5), under a window of 2048 (40 / 8 heads) 350 us
+// (0.87).  Copies issued between the parts of a step instead of together: 531 -> 507 us;
+// exponentials pinned beside the products (the compiler sank them behind): 560 -> 505.
 constexpr int kRing = 4;
 constexpr int kAhead = kRing - 1;
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
@@ -584,6 +589,9 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
 // range with all the queries, through an LDS slot of its own (no workgroup barrier): a
 // stage's operands go to registers as soon as it has landed, and the slot takes the next
 // one.  Two workgroups a CU: 128 KB on their way.  The waves' states are joined at the end.
+// 8 tokens over caches of up to 8192 keys (32 / 8 heads): 23.5 us, 5.4 TB/s, and 7 us to
+// join the ranges; one token that sees 1028 of 16384 keys (40 / 8): 6.5 us, latency (page
+// id, keys, scores, partial sums one after the other), and 5.5 to join.
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
 sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
                      uint16_t* __restrict__ o, float* __restrict__ lse, float* __restrict__ ws_o,
@@ -768,6 +776,7 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
 }
 
 // ---- join the ranges: one wave per (row, q-head), two dims a lane, NB ranges on their way ------
+// (bound by the latency of a launch and two dependent loads: 5.5 to 8.5 us for 1 to 90 rows)
 template <int NB>
 __global__ __launch_bounds__(kThreads) void sf_window_merge_kernel(Call c, int bq,
                                                                    uint16_t* __restrict__ o,
@@ -826,9 +835,14 @@ __global__ __launch_bounds__(kThreads) void sf_window_merge_kernel(Call c, int b
 // over a range of the queries that see them, 32 at a time through an LDS ring: S^T = K Q^T
 // as above, so a lane adds up the weights one of every 32 queries gives to 32 keys, and the
 // lanes are joined every 32 stages, in a fixed order: the error of one fp32 chain over all
-// of them would grow with the queries.  The step of stage i runs the weights of stage i
-// beside S^T of stage i + 1.  Bound by the
-// exponentials (a quarter-rate operation per score) for many rows, by reading K for few.
+// of them would grow with the queries (3e-6 relative for 4096 rows, 1.7e-7 so).  The step
+// of stage i runs the weights of stage i beside S^T of stage i + 1.
+// Many rows: bound by matrix products, weights (an fma, an exponential and an addition per
+// score) and copies in turn on every SIMD: 4096 rows of 28 / 4 heads over themselves 90 us
+// and 4.7 to join the ranges (0.65 PFLOP/s), of which the weights, half the products, the
+// masks or the copies taken away give 8 to 11 us each.  Few rows: latency (page id, K rows,
+// K operands, stages, the lanes' join): 32 rows of 40 / 8 heads over 16416 keys 17 us, 8
+// tokens over 12600 keys in all (32 / 8) 8.5 us.
 struct MassSeq {
   const float* in;
   float* out;
@@ -1231,7 +1245,8 @@ extern "C" int sf_attn_window(const uint16_t* q, const sf_kv_seq* seqs, int n_se
                               float scaling, uint16_t* o, float* lse, void* workspace,
                               size_t workspace_bytes, void* stream) {
   Call c;
-  const int st = make_call(seqs, n_seqs, page_size, block, window, sinks, H, Hkv, hd, scaling, false, c);
+  const int st =
+      make_call(seqs, n_seqs, page_size, block, window, sinks, H, Hkv, hd, scaling, false, c);
   if (st != SF_OK) return st;
   if (c.rows == 0) return SF_OK;
   if (!q || !o || !workspace || !aligned(q) || !aligned(o) || !aligned(workspace))
@@ -1288,7 +1303,8 @@ extern "C" int sf_attn_key_mass(const uint16_t* q, const float* lse, const sf_kv
                                 int Hkv, int hd, float scaling, float decay, void* workspace,
                                 size_t workspace_bytes, void* stream) {
   MassCall c;
-  const int st = make_call(seqs, n_seqs, page_size, block, window, sinks, H, Hkv, hd, scaling, true, c);
+  const int st =
+      make_call(seqs, n_seqs, page_size, block, window, sinks, H, Hkv, hd, scaling, true, c);
   if (st != SF_OK) return st;
   if (!(decay >= 0.f && decay <= 1.f)) return SF_ERR_ARG;
   if (c.rows > 0 && (!q || !lse || !aligned(q))) return SF_ERR_ARG;

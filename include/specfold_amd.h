@@ -557,6 +557,7 @@ int sf_attn_key_mass(const uint16_t* q, const float* lse, const sf_kv_seq* seqs,
  *   mass_out       the kept keys' mass, [l][h] rows at mass_out_layer / _head strides;
  *                  may be NULL; where it is `mass` itself (same strides), entries
  *                  keep .. P - 1 are set to 0; else it overlaps nothing of it
+ *   length_dev, position_dev   int32[1] of the device or NULL: set to keep and to position
  * Keys keep the RoPE angles they were appended with.  Limits: hd == 128, 1 <= P <= 32768,
  * sinks + recent <= keep <= P, keep >= 1; page sizes and alignment as sf_attn_window, a
  * page_table in both; an id outside [0, pages) is read as page 0 and not written.
@@ -574,7 +575,8 @@ typedef struct sf_kv_pages {
 int sf_kv_evict(const float* mass, long long mass_layer, long long mass_head, int layers, int Hkv,
                 int hd, int P, int sinks, int recent, int keep, const sf_kv_pages* from,
                 const sf_kv_pages* to, int32_t* kept, float* mass_out, long long mass_out_layer,
-                long long mass_out_head, void* stream);
+                long long mass_out_head, int32_t* length_dev, int32_t* position_dev, int position,
+                void* stream);
 
 #ifdef __cplusplus
 }

@@ -80,7 +80,7 @@ SIGNATURES = {
     "sf_attn_key_mass": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _f, _vp, _sz,
                               _vp]),
     "sf_kv_evict": (_i, [_vp, _ll, _ll, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _ll, _ll,
-                         _vp]),
+                         _vp, _vp, _i, _vp]),
     "sf_chain_correct": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f,
                               _vp, _vp, _vp, _vp, _vp]),
     "sf_kv_append": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _ll, _ll, _i, _vp]),
@@ -550,13 +550,14 @@ def attn_key_mass(q, lse, batch, li, H, scaling, mass, workspace, mass_in=None, 
 
 
 def kv_evict(mass, length: int, keep: int, sinks: int, recent: int, src, dst, kept,
-             mass_out=None, stream=None) -> None:
+             mass_out=None, position: int = 0, stream=None) -> None:
     """Keep ``keep`` of the first ``length`` keys of every layer and kv head of the paged
     cache ``src`` -- the first ``sinks``, the last ``recent``, then those with the largest
     mass [layers, Hkv, >= length] fp32 -- and move them to the front of ``dst`` (``src``
     itself: in place).  kept [layers, Hkv, keep] int32: their old slots; mass_out [layers,
-    Hkv, >= keep] fp32 (or None; ``mass`` itself: moved in place, the rest zeroed).  The
-    caches' lengths are the caller's (PagedKVCache.evict)."""
+    Hkv, >= keep] fp32 (or None; ``mass`` itself: moved in place, the rest zeroed).
+    ``dst``'s length_dev becomes ``keep`` and its position_dev, where it has one of its own,
+    ``position``; what the host holds of them is the caller's (PagedKVCache.evict)."""
     L, Hkv, hd = src.num_layers, src.Hkv, src.hd
     if (dst.num_layers, dst.Hkv, dst.hd) != (L, Hkv, hd):
         raise ValueError("the caches' layers, kv heads and head sizes differ")
@@ -580,6 +581,7 @@ def kv_evict(mass, length: int, keep: int, sinks: int, recent: int, src, dst, ke
         pages.append(KVPages(c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.page_table.data_ptr(),
                              layer, page, head, c.page_size, c.num_pages))
     none = mass_out is None
+    at = dst.length_dev, dst.position_dev
     layer, head, _ = mass.stride()
     out_layer, out_head, _ = (0, 0, 0) if none else mass_out.stride()
     st = _on_device(load().sf_kv_evict, mass,
@@ -587,7 +589,8 @@ def kv_evict(mass, length: int, keep: int, sinks: int, recent: int, src, dst, ke
                      ("dst", dst.k_pages)), stream,
                     mass.data_ptr(), layer, head, L, Hkv, hd, length, sinks, recent, keep,
                     ctypes.byref(pages[0]), ctypes.byref(pages[1]), kept.data_ptr(),
-                    None if none else mass_out.data_ptr(), out_layer, out_head)
+                    None if none else mass_out.data_ptr(), out_layer, out_head,
+                    at[0].data_ptr(), None if at[1] is at[0] else at[1].data_ptr(), position)
     _check(st, "sf_kv_evict")
 
 

@@ -40,11 +40,15 @@ template <int PER>   // keys of a thread: t = i * 1024 + tid
 __global__ __launch_bounds__(kSelThreads) void sf_evict_select_kernel(
     const float* mass, long long mass_layer, long long mass_head, int Hkv, int P, int sinks,
     int recent, int keep, int32_t* __restrict__ kept, float* mass_out, long long out_layer,
-    long long out_head, int zero_to) {
+    long long out_head, int zero_to, int32_t* length_dev, int32_t* position_dev, int position) {
   __shared__ sf_u32x4 s_hist[kSteps * 64];
   __shared__ int s_cnt[PER * kSelWaves];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int l = blockIdx.x / Hkv, h = blockIdx.x - l * Hkv;
+  if (blockIdx.x == 0 && tid == 0) {   // (two launches fewer for who keeps them)
+    if (length_dev) *length_dev = keep;
+    if (position_dev) *position_dev = position;
+  }
   const float* in = mass + l * mass_layer + h * mass_head;
   const int last = P - recent;
   uint32_t key[PER];
@@ -269,6 +273,7 @@ extern "C" int sf_kv_evict(const float* mass, long long mass_layer, long long ma
                            int layers, int Hkv, int hd, int P, int sinks, int recent, int keep,
                            const sf_kv_pages* from, const sf_kv_pages* to, int32_t* kept,
                            float* mass_out, long long mass_out_layer, long long mass_out_head,
+                           int32_t* length_dev, int32_t* position_dev, int position,
                            void* stream) {
   if (!mass || !kept) return SF_ERR_ARG;
   if (hd != kHD || layers < 1 || Hkv < 1 || P < 1 || P > kMaxKeys) return SF_ERR_SHAPE;
@@ -297,7 +302,8 @@ extern "C" int sf_kv_evict(const float* mass, long long mass_layer, long long ma
 #define SF_EVICT_SELECT(PER)                                                                    \
   hipLaunchKernelGGL((sf_evict_select_kernel<PER>), dim3(layers * Hkv), dim3(kSelThreads), 0, s, \
                      mass, mass_layer, mass_head, Hkv, P, sinks, recent, keep, kept, mass_out,   \
-                     mass_out_layer, mass_out_head, mass_out == mass ? P : 0)
+                     mass_out_layer, mass_out_head, mass_out == mass ? P : 0, length_dev,        \
+                     position_dev, position)
   if (P <= 4 * kSelThreads) SF_EVICT_SELECT(4);
   else if (P <= 16 * kSelThreads) SF_EVICT_SELECT(16);
   else SF_EVICT_SELECT(32);

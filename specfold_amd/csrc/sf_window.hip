@@ -224,7 +224,7 @@ SF_DEV void slow_queries(const uint16_t* q, const Call& c,
         a1 = fmaf(pj, __uint_as_float(w & 0xffff0000u), a1);
       }
     }
-    if (c.nr == 1) {
+    if (keys.nst <= c.spr) {
       *reinterpret_cast<uint32_t*>(out.o + rh * kHD + 2 * lane) = sf_pack2(a0 / l, a1 / l);
       if (out.lse && lane == 0) out.lse[rh] = mx * kLn2 + logf(l);
     } else {
@@ -576,7 +576,7 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
 
   const float l = l_run + __shfl_xor(l_run, 32, 64);
   if (q0 + (lane & 31) >= nq) return;
-  if (c.nr == 1) {
+  if (keys.nst <= c.spr) {
     write_direct(acc, m_ref, l, hf, o + rh * kHD, lse ? lse + rh : nullptr);
   } else {
     const size_t slot = (size_t)it.r * c.rows * c.H + rh;
@@ -767,7 +767,7 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
       }
   }
   if ((lane & 31) >= nq) return;
-  if (c.nr == 1) {
+  if (keys.nst <= c.spr) {
     write_direct(acc, mm, l, hf, o + rh * kHD, lse ? lse + rh : nullptr);
   } else {
     const size_t slot_at = (size_t)it.r * c.rows * c.H + rh;
@@ -796,6 +796,7 @@ __global__ __launch_bounds__(kThreads) void sf_window_merge_kernel(Call c, int b
   const Keys keys =
       query_tile_keys(qi / bq, bq, G, s.rows, s.length, c.block, c.window, c.sinks);
   const int nm = (keys.nst + c.spr - 1) / c.spr;   // <= nr <= 64
+  if (nm == 1) return;   // written by its only range
   const size_t step = (size_t)c.rows * c.H;
   sf_f32x2 a[NB];
   auto load = [&](int r0) {

@@ -80,8 +80,6 @@ class PagedKVCache:
     def _set_length(self, length: int, evicted: int) -> None:
         self.length, self.evicted = length, evicted
         self.length_dev.fill_(length)
-        if evicted and self._position_dev is None:
-            self._position_dev = torch.empty_like(self.length_dev)
         if self._position_dev is not None:
             self._position_dev.fill_(length + evicted)
 
@@ -151,9 +149,12 @@ class PagedKVCache:
         if kept is None:
             kept = torch.empty(self.num_layers, self.Hkv, keep, dtype=torch.int32,
                                device=self.device)
+        position = self.position
+        if position > keep and dst._position_dev is None:
+            dst._position_dev = dst.length_dev.clone()
         _lib.kv_evict(key_mass, self.length, keep, sinks, recent, self, dst, kept,
-                      mass_out=mass_out)
-        dst._set_length(keep, self.position - keep)
+                      mass_out=mass_out, position=position)
+        dst.length, dst.evicted = keep, position - keep   # (on the device: set by the call)
         return kept
 
     def load_dense(self, kv: Sequence[Tuple[torch.Tensor, torch.Tensor]]) -> None:

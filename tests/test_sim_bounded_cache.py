@@ -281,7 +281,7 @@ def _evict(lib, **over):
     f, to = _lib.KVPages(**p), _lib.KVPages(**t)
     return lib.sf_kv_evict(a["mass"], a["ml"], a["mh"], a["layers"], a["Hkv"], a["hd"], a["P"],
                            a["sinks"], a["recent"], a["keep"], ctypes.byref(f), ctypes.byref(to),
-                           a["kept"], a["mass_out"], a["oml"], a["omh"], None)
+                           a["kept"], a["mass_out"], a["oml"], a["omh"], None, None, 0, None)
 
 
 @pytest.mark.parametrize("over,code", [

@@ -524,24 +524,25 @@ def attn_key_mass(q, lse, batch, li, H, scaling, mass, workspace, mass_in=None, 
           min_numel=attn_key_mass_workspace_bytes(batch.num_keys, batch.Hkv))
     if len(mass) != len(seqs) or (mass_in is not None and len(mass_in) != len(seqs)):
         raise ValueError(f"mass, mass_in: one tensor per sequence ({len(seqs)})")
-    dev, Hkv = q.device, batch.Hkv
-    for i, s in enumerate(seqs):
-        t, u = mass[i], None if mass_in is None else mass_in[i]
-        shape, stride, n = t.shape, t.stride(), s.length
-        if t.dtype is not torch.float32 or len(shape) != 2 or shape[0] != Hkv or \
-                shape[1] < n or stride[1] != 1 or t.device != dev:
+    dev, gpu, Hkv, f32 = q.device, q.get_device(), batch.Hkv, torch.float32
+    for s, t, u in zip(seqs, mass, mass if mass_in is None else mass_in):
+        n = s.length
+        if t.dim() != 2:
             raise _bad_mass("mass", t, Hkv, n, dev)
-        s.mass_out, s.mass_out_stride = t.data_ptr(), stride[0]
-        if u is t:
-            s.mass_in, s.mass_in_stride = t.data_ptr(), stride[0]
-        elif u is None:
+        (heads, room), (stride, one) = t.shape, t.stride()
+        if t.dtype is not f32 or heads != Hkv or room < n or one != 1 or t.get_device() != gpu:
+            raise _bad_mass("mass", t, Hkv, n, dev)
+        s.mass_out, s.mass_out_stride = t.data_ptr(), stride
+        if mass_in is None:
             s.mass_in = None
-        else:
-            shape, stride = u.shape, u.stride()
-            if u.dtype is not torch.float32 or len(shape) != 2 or shape[0] != Hkv or \
-                    shape[1] < n or stride[1] != 1 or u.device != dev:
+            continue
+        if u is not t:
+            if u.dim() != 2:
                 raise _bad_mass("mass_in", u, Hkv, n, dev)
-            s.mass_in, s.mass_in_stride = u.data_ptr(), stride[0]
+            (heads, room), (stride, one) = u.shape, u.stride()
+            if u.dtype is not f32 or heads != Hkv or room < n or one != 1 or u.get_device() != gpu:
+                raise _bad_mass("mass_in", u, Hkv, n, dev)
+        s.mass_in, s.mass_in_stride = u.data_ptr(), stride
     st = _on_device(load().sf_attn_key_mass, q,
                     (("lse", lse), ("workspace", workspace), ("caches", batch)), stream,
                     q.data_ptr(), lse.data_ptr(), seqs, len(seqs), batch.page_size, block, window,

@@ -236,10 +236,12 @@ class PagedBatch:
             lengths = None
         now = [c.length for c in self.caches]
         if now != lengths:      # the array holds other lengths than the caches
-            for s, c, n, length in zip(arr, self.caches, self.rows, now):
-                s.rows, s.length = n, length + (n if self.ahead else 0)
-                if s.length > c.capacity:
-                    raise ValueError(f"{s.length} keys exceed the cache's capacity {c.capacity}")
+            keys = [length + n for length, n in zip(now, self.rows)] if self.ahead else now
+            for c, n in zip(self.caches, keys):
+                if n > c.capacity:
+                    raise ValueError(f"{n} keys exceed the cache's capacity {c.capacity}")
+            for s, n, length in zip(arr, self.rows, keys):
+                s.rows, s.length = n, length
             self._layers[li] = arr, views, now
         self.num_keys = sum(now) + (self.num_rows if self.ahead else 0)
         return arr

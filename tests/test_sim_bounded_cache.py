@@ -415,6 +415,18 @@ def test_batch_follows_its_caches(sim):
     assert torch.equal(twice, torch.cat([outs[0], outs[0]]))
     with pytest.raises(ValueError):
         PagedBatch([caches[0], PagedKVCache(1, 2, 64, 64, page_size=16, device="cpu")], [1, 1])
+    # a call refused for lengths past the capacity leaves nothing of them behind
+    c = caches[0]
+    c.length = 38
+    ahead = PagedBatch([c], [2], ahead=True)
+    sim.attn_window(q, ahead, 0, 4, HD ** -0.5, outs[1], ws)
+    c.length = c.capacity
+    with pytest.raises(ValueError):
+        sim.attn_window(q, ahead, 0, 4, HD ** -0.5, outs[1], ws)
+    c.length = 38
+    outs[1].zero_()
+    sim.attn_window(q, ahead, 0, 4, HD ** -0.5, outs[1], ws)
+    assert torch.equal(outs[1], outs[0])
 
 
 def test_mass_of_a_row_without_a_number(sim):

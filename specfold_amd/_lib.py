@@ -152,7 +152,7 @@ def _stream(stream=None):
     if stream is not None:
         return ctypes.c_void_p(stream.cuda_stream)
     # the current stream's handle without a Stream object (which takes 3 us)
-    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, numel: Optional[int] = None,
@@ -161,7 +161,7 @@ def _need(t: torch.Tensor, name: str, dtype: torch.dtype, numel: Optional[int] =
         raise ValueError(f"{name} is required")
     if t.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name}: expected a GPU tensor, got {t.device}")
     if not t.is_contiguous():
         raise ValueError(f"{name}: must be contiguous")
@@ -477,7 +477,7 @@ def _on_device(fn, t: torch.Tensor, others, stream, *args):
     for nm, o in others:
         if o is not None and o.device != dev:
             raise ValueError(f"{nm}: on {o.device}, expected {dev}")
-    if dev.type != "cuda" or dev.index == torch.cuda.current_device():
+    if not t.is_cuda or dev.index == torch._C._cuda_getDevice():
         return fn(*args, _stream(stream))
     with torch.cuda.device(dev):
         return fn(*args, _stream(stream))
@@ -574,13 +574,6 @@ def kv_evict(mass, length: int, keep: int, sinks: int, recent: int, src, dst, ke
                 shape[1] != Hkv or shape[2] < n or t.stride(2) != 1:
             raise ValueError(f"{nm}: expected float32 [{L}, {Hkv}, >= {n}] with contiguous rows, "
                              f"got {t.dtype} {tuple(t.shape)}")
-    pages = []
-    for c in (src, dst):
-        _need(c.k_pages, "k_pages", torch.bfloat16)
-        _need(c.v_pages, "v_pages", torch.bfloat16)
-        layer, page, head = c.k_pages.stride()[:3]
-        pages.append(KVPages(c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.page_table.data_ptr(),
-                             layer, page, head, c.page_size, c.num_pages))
     none = mass_out is None
     at = dst.length_dev, dst.position_dev
     layer, head, _ = mass.stride()
@@ -589,7 +582,7 @@ def kv_evict(mass, length: int, keep: int, sinks: int, recent: int, src, dst, ke
                     (("kept", kept), ("mass_out", mass_out), ("src", src.k_pages),
                      ("dst", dst.k_pages)), stream,
                     mass.data_ptr(), layer, head, L, Hkv, hd, length, sinks, recent, keep,
-                    ctypes.byref(pages[0]), ctypes.byref(pages[1]), kept.data_ptr(),
+                    ctypes.byref(src.pages()), ctypes.byref(dst.pages()), kept.data_ptr(),
                     None if none else mass_out.data_ptr(), out_layer, out_head,
                     at[0].data_ptr(), None if at[1] is at[0] else at[1].data_ptr(), position)
     _check(st, "sf_kv_evict")

@@ -67,6 +67,16 @@ class PagedKVCache:
         self.evicted = 0            # keys dropped by evict
         self._position_dev: Optional[torch.Tensor] = None
 
+    def pages(self):
+        """Every layer's pages, as sf_kv_evict takes them."""
+        k, v, table = self.k_pages, self.v_pages, self.page_table
+        if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or \
+                not k.is_contiguous() or not v.is_contiguous():
+            raise TypeError(f"the pages are contiguous bfloat16, got {k.dtype} and {v.dtype}")
+        layer, page, head = k.stride()[:3]
+        return _lib.KVPages(k.data_ptr(), v.data_ptr(), table.data_ptr(), layer, page, head,
+                            self.page_size, self.num_pages)
+
     # -- positions: the next token's, which an evicted cache's length falls behind ------
     @property
     def position(self) -> int:

@@ -32,6 +32,9 @@ constexpr int kMaxH = 256;   // (a sequence's rows of q: 32-bit byte offsets)
 constexpr int kThreads = 256;
 constexpr int kCUs = 256;
 constexpr int kTileQ = 128;   // queries of a tile
+// Few queries: tiles of 9 to 36 stages go to eight waves and one range, if there are no more
+// of them than CUs (a workgroup's LDS fills one).
+constexpr int kWideLeast = 9, kWideMost = 36;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLazy = 8.f;   // base-2 headroom of the softmax reference
@@ -77,6 +80,7 @@ struct Call {
   Seq s[kMaxSeqs];
   int n_seqs, page_shift, block, window, sinks, H, Hkv, rows;
   int tiles, nr, spr;      // tiles of all sequences, ranges of a tile, stages of a range
+  int longest;             // stages of the longest tile
 };
 
 SF_DEV int page_in(const Seq& s, int id) { return id >= 0 && id < s.pages ? id : 0; }
@@ -585,19 +589,26 @@ sf_window_tile_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
 }
 
 // ---- up to 32 queries of a kv head (a token, or a few) ---------------------------------------
-// Bound by reading the cache once: each of the four waves takes every fourth stage of the
+// Bound by reading the cache once: each of the W waves takes every W-th stage of the
 // range with all the queries, through an LDS slot of its own (no workgroup barrier): a
 // stage's operands go to registers as soon as it has landed, and the slot takes the next
-// one.  Two workgroups a CU: 128 KB on their way.  The waves' states are joined at the end.
+// one.  Four waves, two workgroups a CU, or eight waves and one: 128 KB on their way.  The
+// waves' states are joined at the end.  Eight waves take a tile's stages without ranges, so
+// without their join: one token of a cache (32 / 8 heads), ranges and join against eight
+// waves: 7 stages 7.3 / 7.3 us, 13 9.8 / 8.6, 19 10.5 / 9.2, 26 10.5 / 10.5, 33 10.6 / 11.9
+// (eight sequences: 12.9 / 12.0; a launch less, 4 us of the host, on this side), 41 10.7 /
+// 13.4.
 // 8 tokens over caches of up to 8192 keys (32 / 8 heads): 23.5 us, 5.4 TB/s, and 7 us to
-// join the ranges; one token that sees 1028 of 16384 keys (40 / 8): 6.5 us, latency (page
-// id, keys, scores, partial sums one after the other), and 5.5 to join.
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+// join the ranges; one token that sees 1028 of 16384 keys (40 / 8): 12 us of eight waves,
+// latency: page id, then five rounds of keys.
+template <int W>   // waves
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void
 sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
                      uint16_t* __restrict__ o, float* __restrict__ lse, float* __restrict__ ws_o,
                      float* __restrict__ ws_ml) {
-  __shared__ __attribute__((aligned(16))) uint8_t ring[4 * kSlot];
-  __shared__ int s_bad[4];
+  __shared__ __attribute__((aligned(16))) uint8_t ring[W * kSlot];
+  __shared__ int s_bad[W];
+  __shared__ sf_f32x2 s_ml[W][32];
   const Item it = find_item<true>(c);
   const Seq& s = c.s[it.si];
   const int lane = threadIdx.x & 63, hf = lane >> 5;
@@ -610,7 +621,7 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   const int lastg = last_group(P);
   // lane i: 16-key group i & 1 of this wave's stage 32u + i / 2 (past the range: the last)
   auto lane_group = [&](int u) {
-    return min(keys.key0(c0 + min(wv + 4 * (32 * u + (lane >> 1)), nst - 1)) + 16 * (lane & 1),
+    return min(keys.key0(c0 + min(wv + W * (32 * u + (lane >> 1)), nst - 1)) + 16 * (lane & 1),
                lastg);
   };
   auto load_pages = [&](int u) { return s.table ? s.table[lane_group(u) >> c.page_shift] : 0; };
@@ -634,7 +645,7 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   auto issue = [&](int j) {   // this wave's stage j
     if (j > 0 && (j & 31) == 0)
       groups.set(group_off(s, c.page_shift, load_pages(j >> 5), lane_group(j >> 5)));
-    const int key0 = keys.key0(c0 + wv + 4 * j);
+    const int key0 = keys.key0(c0 + wv + W * j);
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const int last = min(15, P - 1 - min(key0 + 16 * g, lastg));   // of the group's rows
@@ -665,7 +676,7 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
     for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
 
 #pragma unroll 1
-  for (int j = 0; wv + 4 * j < nst; ++j) {
+  for (int j = 0; wv + W * j < nst; ++j) {
     wait_vm_wave<0>();   // the stage (and the queries) have landed
     sf_u32x4 kf[8];
     sf_u32x2 vf[16];
@@ -674,14 +685,14 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
     sf_lds_reads_done(kf);
     sf_lds_reads_done(vf);
     wait_vm_wave<63>();   // (every lane has read)
-    if (wv + 4 * (j + 1) < nst) issue(j + 1);
+    if (wv + W * (j + 1) < nst) issue(j + 1);
     sf_f32x16 sc;
 #pragma unroll
     for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks)
       sc = mfma32(sf_as_bf16x8(kf[ks]), sf_as_bf16x8(qf[ks]), sc);
-    const int key0 = keys.key0(c0 + wv + 4 * j);
+    const int key0 = keys.key0(c0 + wv + W * j);
     const bool masked = key0 + kStage > end_min || (key0 < lo_max && key0 + kStage > c.sinks);
     if (masked) mask_scores(sc, key0, hf, end, lo, c.sinks);
     float mx = sc[0];
@@ -715,64 +726,64 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
   // a hidden value that was not finite: the item again, a key at a time
   if (lane == 0) s_bad[wv] = bad;
   __syncthreads();
-  if (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) {   // workgroup-uniform
-    slow_queries(q, c, s, it.h, it.r, 8 * wv, 8, keys, c0, nst,
+  int any = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) any |= s_bad[w];
+  if (any) {   // workgroup-uniform
+    slow_queries(q, c, s, it.h, it.r, 32 / W * wv, 32 / W, keys, c0, nst,
                  Out{o, lse, ws_o, ws_ml, scale_log2});
     return;
   }
 
-  // join the four waves' states: waves 1..3 leave theirs in LDS
-  float* xo = reinterpret_cast<float*>(ring);           // [wave - 1][dt][4][lane] x 4
-  float* xml = xo + 3 * 4 * 4 * 64 * 4;                 // [wave - 1][query] x 2
-  if (wv > 0) {
+  // join the waves' states through LDS, each wave 16 / W of the 16 pieces of the dims
+  float* const xo = reinterpret_cast<float*>(ring);   // [wave][dt][4][lane] x 4
 #pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
+  for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        *reinterpret_cast<sf_f32x4*>(xo + ((((wv - 1) * 4 + dt) * 4 + b) * 64 + lane) * 4) =
-            sf_f32x4{acc[dt][4 * b], acc[dt][4 * b + 1], acc[dt][4 * b + 2],
-                     acc[dt][4 * b + 3]};
-    if (hf == 0) {
-      xml[((wv - 1) * 32 + lane) * 2] = m_ref;
-      xml[((wv - 1) * 32 + lane) * 2 + 1] = l_run;
-    }
-  }
+    for (int b = 0; b < 4; ++b)
+      *reinterpret_cast<sf_f32x4*>(xo + (((wv * 4 + dt) * 4 + b) * 64 + lane) * 4) =
+          sf_f32x4{acc[dt][4 * b], acc[dt][4 * b + 1], acc[dt][4 * b + 2], acc[dt][4 * b + 3]};
+  if (hf == 0) s_ml[wv][lane] = sf_f32x2{m_ref, l_run};
   __syncthreads();
-  if (wv > 0) return;
-  float mm = m_ref;
-  float mw[3], lw[3];
+  float f[W], mm = -INFINITY, l = 0.f;
+  sf_f32x2 ml[W];
 #pragma unroll
-  for (int w = 0; w < 3; ++w) {
-    mw[w] = xml[(w * 32 + (lane & 31)) * 2];
-    lw[w] = xml[(w * 32 + (lane & 31)) * 2 + 1];
-    mm = fmaxf(mm, mw[w]);
+  for (int w = 0; w < W; ++w) {
+    ml[w] = s_ml[w][lane & 31];
+    mm = fmaxf(mm, ml[w].x);
   }
   const float mu = mm == -INFINITY ? 0.f : mm;
-  const float w0 = __builtin_amdgcn_exp2f(m_ref - mu);
-  float l = l_run * w0;
 #pragma unroll
-  for (int dt = 0; dt < 4; ++dt) acc[dt] = acc[dt] * w0;
-#pragma unroll
-  for (int w = 0; w < 3; ++w) {
-    const float f = __builtin_amdgcn_exp2f(mw[w] - mu);
-    l += lw[w] * f;
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const sf_f32x4 x = *reinterpret_cast<const sf_f32x4*>(
-            xo + (((w * 4 + dt) * 4 + b) * 64 + lane) * 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[dt][4 * b + i] = fmaf(x[i], f, acc[dt][4 * b + i]);
-      }
+  for (int w = 0; w < W; ++w) {
+    f[w] = __builtin_amdgcn_exp2f(ml[w].x - mu);
+    l = fmaf(ml[w].y, f[w], l);
   }
   if ((lane & 31) >= nq) return;
-  if (keys.nst <= c.spr) {
-    write_direct(acc, mm, l, hf, o + rh * kHD, lse ? lse + rh : nullptr);
-  } else {
-    const size_t slot_at = (size_t)it.r * c.rows * c.H + rh;
-    write_partial(acc, mm, l, hf, ws_o + slot_at * kHD, ws_ml + slot_at * 2);
+  const bool direct = keys.nst <= c.spr;
+  const size_t slot_at = direct ? 0 : (size_t)it.r * c.rows * c.H + rh;
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int u = 0; u < 16 / W; ++u) {
+    const int piece = 16 / W * wv + u, dim = 8 * piece + 4 * hf;
+    sf_f32x4 x{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const sf_f32x4 y =
+          *reinterpret_cast<const sf_f32x4*>(xo + ((w * 16 + piece) * 64 + lane) * 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = fmaf(y[i], f[w], x[i]);
+    }
+    if (direct)
+      *reinterpret_cast<sf_u32x2*>(o + rh * kHD + dim) =
+          sf_u32x2{sf_pack2(x[0] * inv, x[1] * inv), sf_pack2(x[2] * inv, x[3] * inv)};
+    else
+      sf_handoff_store(reinterpret_cast<sf_f32x4*>(ws_o + slot_at * kHD + dim), x);
   }
+  if (wv > 0 || hf > 0) return;
+  if (!direct)
+    sf_handoff_store(reinterpret_cast<sf_f32x2*>(ws_ml + slot_at * 2), sf_f32x2{mm, l});
+  else if (lse)
+    lse[rh] = mm * kLn2 + logf(l);
 }
 
 // ---- join the ranges: one wave per (row, q-head), two dims a lane, NB ranges on their way ------
@@ -1229,6 +1240,7 @@ int plan_ranges(Call& c, int bq, int least, int most, int slots, Cost fix, int u
     }
   }
   if (c.tiles == 0) return 0;
+  c.longest = longest;
   plan_spread(c, work, longest, ranges_cap(c.rows), slots, fix, unit);
   return c.tiles * c.nr * c.Hkv;
 }
@@ -1274,13 +1286,23 @@ extern "C" int sf_attn_window(const uint16_t* q, const sf_kv_seq* seqs, int n_se
   const int few_most = others && few_stages * Hkv < 3500 ? 0 : 32;
   for (int few = 1; few >= 0; --few) {
     const int bq = few ? 32 : kTileQ;
-    const int items =
+    int items =
         few ? plan_ranges(c, bq, 1, few_most, 2 * kCUs, Cost{12, 20}, 4)
             : plan_ranges(c, bq, few_most + 1, 1 << 30, 2 * kCUs, Cost{6, 24}, 1);
     if (items == 0) continue;
-    if (few)
-      hipLaunchKernelGGL(sf_window_few_kernel, dim3(items), dim3(kThreads), 0, hs, q, c,
-                         scale_log2, o, lse, ws_o, ws_ml);
+    const int longest = c.longest;
+    const bool wide = few && c.tiles * Hkv <= kCUs && longest >= kWideLeast && longest <= kWideMost;
+    if (wide) {   // all of a tile's stages
+      c.nr = 1;
+      c.spr = longest;
+      items = c.tiles * Hkv;
+    }
+    if (few && wide)
+      hipLaunchKernelGGL(sf_window_few_kernel<8>, dim3(items), dim3(512), 0, hs, q, c, scale_log2,
+                         o, lse, ws_o, ws_ml);
+    else if (few)
+      hipLaunchKernelGGL(sf_window_few_kernel<4>, dim3(items), dim3(256), 0, hs, q, c, scale_log2,
+                         o, lse, ws_o, ws_ml);
     else
       hipLaunchKernelGGL(sf_window_tile_kernel, dim3(items), dim3(kThreads), 0, hs, q, c,
                          scale_log2, o, lse, ws_o, ws_ml);

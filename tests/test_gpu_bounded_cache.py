@@ -35,6 +35,11 @@ WINDOW = [
     ([(700, 1500)], 7, 7, 1, 1, 0, 16),
     ([(600, 1800)], 16, 1, 16, 200, 130, 16),
     ([(2047, 2111)], 28, 4, 64, 1000, 1, 128),
+    # (few queries over 9 to 36 stages of keys, and just outside)
+    ([(1, p) for p in (1151, 289, 288, 257, 256, 33, 1, 1152)], 32, 8, 1, 0, 0, 16),
+    ([(1, 1152), (1, 1153)], 40, 8, 1, 0, 0, 16),
+    ([(2, 1030), (3, 900)], 40, 8, 1, 500, 70, 32),
+    ([(2, 900)], 16, 1, 2, 0, 0, 128),
 ]
 
 
@@ -54,7 +59,8 @@ def test_window_large_scores(shapes, H, Hkv, block):
 @pytest.mark.parametrize("n,P,block,window,sinks,at", [
     (64, 64, 32, 0, 0, 40), (1000, 1077, 1, 0, 0, 600), (1024, 2048, 32, 256, 4, 1500),
     (200, 5200, 16, 0, 0, 5199), (129, 129, 64, 0, 0, 128), (700, 900, 1, 100, 40, 330),
-    (2, 3000, 1, 0, 0, 2999), (32, 4000, 32, 100, 4, 3880)])
+    (2, 3000, 1, 0, 0, 2999), (32, 4000, 32, 100, 4, 3880), (2, 500, 1, 0, 0, 499),
+    (2, 900, 1, 300, 4, 599)])
 @pytest.mark.parametrize("bad", [float("inf"), float("nan")])
 def test_hidden_key_not_finite(n, P, block, window, sinks, at, bad):
     """A value or key that is not finite reaches the rows that see it (a value: in its

@@ -39,6 +39,8 @@ WINDOW = [
     ([(64, 64)], 4, 4, 64, 500, 2, 16),                # a window wider than all
     ([(20, 60)], 16, 1, 4, 7, 1, 16),                  # 16 heads a kv head
     ([(130, 131), (67, 300)], 5, 1, 32, 100, 2, 16),
+    ([(1, 400), (2, 520), (1, 30), (0, 9)], 8, 2, 1, 0, 0, 16),   # few queries, more stages
+    ([(3, 700)], 4, 2, 2, 350, 20, 64),
 ]
 
 
@@ -67,7 +69,8 @@ def test_window_contiguous(sim):
 # that others of the tile see
 @pytest.mark.parametrize("n,P,block,window,sinks,at", [
     (64, 64, 32, 0, 0, 40), (70, 220, 1, 0, 0, 200), (70, 220, 1, 30, 0, 155),
-    (70, 400, 32, 64, 5, 300), (40, 300, 8, 100, 3, 2), (2, 130, 1, 0, 0, 129)])
+    (70, 400, 32, 64, 5, 300), (40, 300, 8, 100, 3, 2), (2, 130, 1, 0, 0, 129),
+    (2, 400, 1, 0, 0, 399), (3, 400, 1, 300, 4, 99)])
 @pytest.mark.parametrize("bad", [float("inf"), float("nan")])
 def test_hidden_key_not_finite(sim, n, P, block, window, sinks, at, bad):
     H, Hkv = 4, 2

@@ -787,7 +787,7 @@ sf_window_few_kernel(const uint16_t* __restrict__ q, Call c, float scale_log2,
 }
 
 // ---- join the ranges: one wave per (row, q-head), two dims a lane, NB ranges on their way ------
-// (bound by the latency of a launch and two dependent loads: 5.5 to 8.5 us for 1 to 90 rows)
+// (bound by the latency of a launch and two dependent loads: 5.5 to 8 us for 1 to 90 rows)
 template <int NB>
 __global__ __launch_bounds__(kThreads) void sf_window_merge_kernel(Call c, int bq,
                                                                    uint16_t* __restrict__ o,
